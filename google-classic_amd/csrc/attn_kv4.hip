@@ -1,0 +1,376 @@
+// attn_kv4.hip -- attention over the 4-bit cache (holo_attention_kv4).
+//
+// softmax(q . k_p / sqrt(hd)) . v_p over the positions p a row sees, for the last
+// rows of several sequences.  Both products run on v_mfma_f32_16x16x32_f16,
+// transposed: S^T = K Q^T and O^T = V^T P^T, so that a lane holds one column (a
+// query row and head) throughout.
+//   - The columns of a KV head are its entry's rows times the query heads that
+//     share it, 16 of them a tile: all the heads of a grouped-query decode step
+//     at once.
+//   - A cached value d * c is an exact f16 (kv4.h, holo_forward.h): a code's
+//     four bits shifted into an f16's mantissa under the exponent of 16 are 16 +
+//     c + 8, and one packed fma with d and -24 d makes d * c of it.
+//   - q (scaled by a power of two to its row's largest value) and the
+//     probabilities are two f16 halves, x - hi - lo within 2^-22 |x|: fp32's
+//     class with two matrix instructions.  Probabilities are held times 2^8, so
+//     that a small one's lo stays above f16's smallest step.
+//   - The softmax is one pass: the running maximum of a column moves only when a
+//     score passes it by 2^7 (p then stays below 2^15), which few tiles do.
+//   - A lane's scores are those of the eight positions that its V words hold:
+//     P is the second product's operand without crossing lanes.
+// A workgroup's waves take the tiles of a range in turn and meet in LDS; ranges
+// of a long sequence are workgroups of their own, whose partial sums a second
+// launch joins in range order.
+#include "attn_tiles.h"
+#include "kv4.h"
+#include "stream_scratch.h"
+
+#include <float.h>
+
+namespace holo {
+
+// The 8 values of a word as an MFMA operand; d and d24 = -24 d of the pairs (2 p, 2 p + 1).
+__device__ __forceinline__ h8 kv4_unpack(uint32_t w, const h2 d[4], const h2 d24[4])
+{
+    h2 x[4];
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+        const uint32_t n = p < 2 ? w << (6 - 4 * p) : w >> (4 * p - 6);
+        x[p] = __builtin_elementwise_fma(__builtin_bit_cast(h2, (n & 0x03C003C0u) | 0x4C004C00u), d[p], d24[p]);
+    }
+    return h8{x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
+}
+
+// A tile in a lane's registers.
+template <int NB>
+struct Tile {
+    uint32_t k[2][NB], v[2 * NB];
+    uint16_t ks[2][NB];  // the scale of each K word's block
+    u4 vs[NB];
+};
+
+template <int NB>
+__device__ __forceinline__ void load_tile(Tile<NB> &t, const uint8_t *at, int lane)
+{
+    constexpr int HD = 32 * NB, W = NB % 2 ? 2 : 4;
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint32_t *k = (const uint32_t *)at + (64 * h + lane) * NB;
+        if constexpr (NB == 4) *(u4 *)t.k[h] = *(const u4 *)k;
+        else if constexpr (NB == 2) *(uint2 *)t.k[h] = *(const uint2 *)k;
+        else
+#pragma unroll
+            for (int j = 0; j < NB; j++) t.k[h][j] = k[j];
+    }
+    const uint32_t *v = (const uint32_t *)(at + 16 * HD);
+#pragma unroll
+    for (int c = 0; c < 2 * NB / W; c++) {
+        if constexpr (W == 4) *(u4 *)(t.v + 4 * c) = *(const u4 *)(v + (64 * c + lane) * 4);
+        else *(uint2 *)(t.v + 2 * c) = *(const uint2 *)(v + (64 * c + lane) * 2);
+    }
+    const uint32_t *ks = (const uint32_t *)(at + 32 * HD);
+#pragma unroll
+    for (int j = 0; j < NB; j++) {
+        const uint32_t s = ks[16 * ((NB * g + j) >> 2) + r];
+        t.ks[0][j] = (uint16_t)s;
+        t.ks[1][j] = (uint16_t)(s >> 16);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++) t.vs[b] = *(const u4 *)(at + 34 * HD + 64 * b + 16 * g);
+}
+
+struct Kv4Attn {
+    Kv4View c;
+    holo_batch_t b;
+    float *out, *part;
+    const float *q;
+    int ldo, ldq, n_heads;
+    int chunk;   // tiles of a range
+    int splits;  // ranges a sequence of max_len positions has
+    int ctiles;  // tiles of 16 columns that max_rows rows have
+};
+
+// Column c of an entry and KV head: row c / G, query head kvh * G + c % G.
+// Waves: W; the columns of a workgroup: 16.
+template <int NB, int W>
+__global__ __launch_bounds__(64 * W) void attn_kv4_k(Kv4Attn a)
+{
+    constexpr int HD = 32 * NB, OS = HD + 4;
+    __shared__ __align__(16) float lo_[W][16][OS];
+    __shared__ float lm[W][16], ll[W][16];
+    const int kvh = blockIdx.y / a.ctiles, ct = blockIdx.y % a.ctiles;
+    const int G = a.n_heads / a.c.n_kv_heads;
+    const Kv4Entry e = kv4_entry(a.c, a.b, blockIdx.z);
+    const int ncols = e.take * G, c0 = 16 * ct;
+    if (c0 >= ncols) return;
+    const bool too_long = e.len > a.b.max_len;
+    // the tiles that the tile's last row sees, in ranges
+    const int last_row = (min(c0 + 16, ncols) - 1) / G, first_row = c0 / G;
+    const int from = e.len - e.rows;
+    const int see = max(from + last_row + 1, 0);  // positions the last row sees
+    const int ntiles = too_long ? 0 : (see + 31) >> 5;
+    const int t0 = blockIdx.x * a.chunk, t1 = min(t0 + a.chunk, ntiles);
+    if (t0 >= ntiles && blockIdx.x > 0) return;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int col = c0 + r;
+    const bool valid = col < ncols;
+    const int row = valid ? col / G : 0, head = kvh * G + (valid ? col % G : 0);
+    const int qpos = valid ? from + row : -1;  // the column sees positions 0 .. qpos
+    const int all = from + first_row;          // positions 0 .. all are seen by every column
+
+    // q of the column: dims 8 (NB g + j) .. + 7 in step j, scaled to [2^13, 2^14)
+    h8 qh[NB], ql[NB];
+    float sc;
+    {
+        float x[NB][8], big = 0.f;
+        const float *qp = a.q + (int64_t)(e.first + row) * a.ldq + (int64_t)head * HD + 8 * NB * g;
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            const float4 u = valid ? *(const float4 *)(qp + 8 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 w = valid ? *(const float4 *)(qp + 8 * j + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[j][0] = u.x, x[j][1] = u.y, x[j][2] = u.z, x[j][3] = u.w;
+            x[j][4] = w.x, x[j][5] = w.y, x[j][6] = w.z, x[j][7] = w.w;
+#pragma unroll
+            for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[j][i]));
+        }
+        big = fmaxf(big, __shfl_xor(big, 16, 64));
+        big = fmaxf(big, __shfl_xor(big, 32, 64));
+        // rows of zeros, and rows with an infinity (whose halves make NaN of it), as they are
+        const int ex = big > 0.f && big <= FLT_MAX ? ilogbf(big) - 13 : 0;
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[j][i] = ldexpf(x[j][i], -ex);
+            split8(x[j], qh[j], ql[j]);
+        }
+        sc = ldexpf(1.4426950408889634f / sqrtf((float)HD), ex);
+    }
+
+    float m = -FLT_MAX, l = 0.f;  // of log2 units; l: this lane's positions
+    f4 o[2 * NB];
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) o[i] = f4{};
+
+    for (int t = t0 + wave; t < t1; t += W) {
+        const uint8_t *at = kv4_tile<NB>(a.c, e, kvh, t);
+        if (!at) continue;  // no page: positions that nobody sees
+        Tile<NB> x;
+        load_tile<NB>(x, at, lane);
+        f4 s[2] = {f4{}, f4{}};
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                const _Float16 d = __builtin_bit_cast(_Float16, x.ks[h][j]);
+                const h2 dd = {d, d}, dm = dd * (_Float16)-24.f;
+                const h2 d4[4] = {dd, dd, dd, dd}, m4[4] = {dm, dm, dm, dm};
+                const h8 k8 = kv4_unpack(x.k[h][j], d4, m4);
+                s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[j], s[h], 0, 0, 0);
+                s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[j], s[h], 0, 0, 0);
+            }
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = s[i >> 2][i & 3] * sc;
+        const int p0 = 32 * t;
+        if (p0 + 31 > all) {
+            // some column does not see the whole tile.  Its probability is 0 where it
+            // does not; the values there must be finite then: a scale past the end, or a NaN
+            // that some column does not see, becomes 0, and a column that sees the NaN
+            // takes it here.
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int pos = p0 + v_pos(g, i);
+                if (pos > qpos) p[i] = -INFINITY;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                h8 d = __builtin_bit_cast(h8, x.vs[b]);
+                int nan = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int pos = p0 + v_pos(g, i);
+                    const bool is = d[i] != d[i];
+                    nan |= is && pos <= qpos;
+                    if (pos >= e.len || (is && pos > all)) d[i] = (_Float16)0.f;
+                }
+                x.vs[b] = __builtin_bit_cast(u4, d);
+                nan |= __shfl_xor(nan, 16, 64);
+                nan |= __shfl_xor(nan, 32, 64);
+                if (nan) o[2 * b] = o[2 * b + 1] = f4{NAN, NAN, NAN, NAN};
+            }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+        if (__any(mx > m + kMaxSlack)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
+            const float w = __builtin_amdgcn_exp2f(m - mx);
+            m = mx;
+            l *= w;
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) o[i] *= w;
+        }
+        float ps = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            p[i] = __builtin_amdgcn_exp2f(p[i] - m + kPShift);
+            ps += p[i];
+        }
+        l += ps;
+        h8 ph, pl;
+        split8(p, ph, pl);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            h2 d4[4], m4[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                d4[i] = __builtin_bit_cast(h2, (uint32_t)x.vs[b][i]);
+                m4[i] = d4[i] * (_Float16)-24.f;
+            }
+#pragma unroll
+            for (int i = 2 * b; i < 2 * b + 2; i++) {
+                const h8 v8 = kv4_unpack(x.v[i], d4, m4);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[i], 0, 0, 0);
+            }
+        }
+    }
+
+    // the waves meet: O = sum_w 2^(m_w - M) O_w
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) *(f4 *)&lo_[wave][r][16 * i + 4 * g] = o[i];
+    if (g == 0) {
+        lm[wave][r] = m;
+        ll[wave][r] = l;
+    }
+    __syncthreads();
+    // one range: the entry's tiles are all here
+    const bool whole = a.splits == 1 || ntiles <= a.chunk;
+    for (int i = threadIdx.x; i < 16 * (HD / 4); i += 64 * W) {
+        const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
+        if (c0 + c >= ncols) continue;
+        float M = lm[0][c];
+#pragma unroll
+        for (int w = 1; w < W; w++) M = fmaxf(M, lm[w][c]);
+        float L = 0.f;
+        f4 O = f4{};
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float f = __builtin_amdgcn_exp2f(lm[w][c] - M);
+            L = fmaf(f, ll[w][c], L);
+            O += f * *(const f4 *)&lo_[w][c][d];
+        }
+        const int64_t at = e.first + (c0 + c) / G;
+        const int h = kvh * G + (c0 + c) % G;
+        if (whole) {
+            // a row that sees nothing gives zeros (a NaN that it sees is in its sums)
+            const float f = L == 0.f ? 0.f : 1.0f / L;
+            f4 y = O * f;
+            if (too_long) y = f4{NAN, NAN, NAN, NAN};
+            *(f4 *)(a.out + at * a.ldo + (int64_t)h * HD + d) = y;
+        } else {
+            float *pp = a.part + ((at * a.n_heads + h) * a.splits + blockIdx.x) * (HD + 4);
+            *(f4 *)(pp + d) = O;
+            if (d == 0) *(f2 *)(pp + HD) = f2{M, L};
+        }
+    }
+}
+
+// Joins the ranges of a row and head, in range order.
+template <int NB>
+__global__ __launch_bounds__(64) void attn_kv4_join_k(Kv4Attn a)
+{
+    constexpr int HD = 32 * NB, D = HD / 4;  // a lane's four dims
+    const Kv4Entry e = kv4_entry(a.c, a.b, blockIdx.z);
+    const int h = blockIdx.x, row = blockIdx.y;
+    if (row >= e.take || e.len > a.b.max_len) return;
+    const int G = a.n_heads / a.c.n_kv_heads;
+    // the ranges of the row's tile of columns, as the workgroups above have it
+    const int c0 = (row * G + h % G) & ~15, last_row = (min(c0 + 16, e.take * G) - 1) / G;
+    const int ntiles = (max(e.len - e.rows + last_row + 1, 0) + 31) >> 5;
+    const int n = (ntiles + a.chunk - 1) / a.chunk;
+    if (n <= 1) return;
+    const int64_t at = e.first + row;
+    const float *pp = a.part + ((at * a.n_heads + h) * a.splits) * (HD + 4);
+    float M = -FLT_MAX;
+    for (int s = 0; s < n; s++) M = fmaxf(M, pp[s * (HD + 4) + HD]);
+    if (threadIdx.x >= D) return;
+    float L = 0.f;
+    f4 O = f4{};
+    for (int s = 0; s < n; s++) {
+        const float f = __builtin_amdgcn_exp2f(pp[s * (HD + 4) + HD] - M);
+        L = fmaf(f, pp[s * (HD + 4) + HD + 1], L);
+        O += f * *(const f4 *)(pp + s * (HD + 4) + 4 * threadIdx.x);
+    }
+    *(f4 *)(a.out + at * a.ldo + (int64_t)h * HD + 4 * threadIdx.x) = O * (L == 0.f ? 0.f : 1.0f / L);
+}
+
+// Tiles of a range: all of a sequence where the launch has two workgroups a CU
+// without ranges, else as many ranges as bring it there, of at least 4 tiles.
+static int range_tiles(int64_t groups, int tiles)
+{
+    const int64_t want = (2 * (int64_t)num_cus() + groups - 1) / groups;
+    const int64_t chunk = (tiles + want - 1) / want;
+    return (int)(chunk < 4 ? 4 : chunk);
+}
+
+template <int NB>
+static int run_attn(Kv4Attn a)
+{
+    constexpr int W = 4;
+    const int G = a.n_heads / a.c.n_kv_heads, take = a.b.max_rows;
+    a.ctiles = (int)(((int64_t)take * G + 15) / 16);
+    const int tiles = (a.b.max_len + 31) / 32;
+    const int64_t groups = (int64_t)a.ctiles * a.c.n_kv_heads * a.b.n_seqs;
+    a.chunk = range_tiles(groups, tiles);
+    a.splits = max(1, (tiles + a.chunk - 1) / a.chunk);
+    const dim3 grid(a.splits, a.ctiles * a.c.n_kv_heads, a.b.n_seqs);
+    if (a.splits == 1) {
+        hipLaunchKernelGGL((attn_kv4_k<NB, W>), grid, dim3(64 * W), 0, stream(), a);
+        HOLO_LAUNCH_CHECK();
+        return 0;
+    }
+    const StreamScratch scratch((size_t)a.b.rows * a.n_heads * a.splits * (32 * NB + 4) * sizeof(float));
+    a.part = (float *)scratch.get();
+    if (!a.part) {
+        latch_error((int)hipErrorOutOfMemory, "holo_attention_kv4: partial sums", __FILE__, __LINE__);
+        return (int)hipErrorOutOfMemory;
+    }
+    hipLaunchKernelGGL((attn_kv4_k<NB, W>), grid, dim3(64 * W), 0, stream(), a);
+    HOLO_LAUNCH_CHECK();
+    hipLaunchKernelGGL(attn_kv4_join_k<NB>, dim3(a.n_heads, take, a.b.n_seqs), dim3(64), 0, stream(), a);
+    HOLO_LAUNCH_CHECK();
+    return 0;
+}
+
+}  // namespace holo
+
+using namespace holo;
+
+extern "C" int holo_attention_kv4(const holo_kv4_t *c, int layer, float *out, const float *q, int ldo, int ldq,
+                                  int n_heads, const holo_batch_t *b)
+{
+    if (!kv4_call_ok(c, layer, b) || n_heads <= 0 || n_heads % c->n_kv_heads != 0) {
+        HOLO_REJECT("holo_attention_kv4: cache, layer, heads or batch outside the supported set");
+        return HOLO_EINVAL;
+    }
+    if (b->rows == 0 || b->n_seqs == 0) return 0;
+    const int64_t dim = (int64_t)n_heads * c->head_dim;
+    Kv4Attn a{kv4_view(c, layer), *b, out, nullptr, q, ldo, ldq, n_heads, 0, 0, 0};
+    a.b.max_rows = b->max_rows < b->rows ? b->max_rows : b->rows;
+    const int64_t cols = (int64_t)a.b.max_rows * (n_heads / c->n_kv_heads);
+    if (!rows_ok(q, ldq, dim) || !rows_ok(out, ldo, dim) || b->max_len < 0 || b->max_len > 0x7FFFF000 ||
+        (cols + 15) / 16 * c->n_kv_heads > 65535 || a.b.max_rows > 65535) {
+        HOLO_REJECT("holo_attention_kv4: null or misaligned rows, rows that overlap, or more rows than one launch takes");
+        return HOLO_EINVAL;
+    }
+    switch (c->head_dim) {
+    case 32: return run_attn<1>(a);
+    case 64: return run_attn<2>(a);
+    case 96: return run_attn<3>(a);
+    default: return run_attn<4>(a);
+    }
+}

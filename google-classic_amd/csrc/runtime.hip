@@ -34,7 +34,9 @@ void latch_error(int code, const char *what, const char *file, int line)
 {
     int expected = 0;
     g_error.compare_exchange_strong(expected, code);
-    const char *msg = code == HOLO_EINVAL ? "invalid argument" : hipGetErrorString((hipError_t)code);
+    const char *msg = code == HOLO_EINVAL     ? "invalid argument"
+                      : code == HOLO_ENOPAGES ? "not enough free pages"
+                                              : hipGetErrorString((hipError_t)code);
     fprintf(stderr, "holo_mi355x error %d (%s) at %s:%d: %s\n", code, msg, file, line, what);
 }
 
@@ -81,6 +83,7 @@ const char *holo_error_string(int code)
 {
     if (code == 0) return "ok";
     if (code == HOLO_EINVAL) return "invalid argument";
+    if (code == HOLO_ENOPAGES) return "not enough free pages";
     if (code == HOLO_ECHAIN) return "persistent decode-step launch could not synchronise its workgroups";
     return hipGetErrorString((hipError_t)code);
 }

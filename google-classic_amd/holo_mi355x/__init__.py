@@ -193,12 +193,28 @@ _SIGS = {
     "holo_llama_release": (None, [_P]),
     "holo_llama_from_gguf": (_I, [_P, _P, _P, _I]),
     "holo_llama_gguf_check": (_I, [_P]),
+    # several sequences at once, the 4-bit cache (include/holo_forward.h)
+    "holo_attention_packed": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "holo_kv4_page_bytes": (_SZ, [_P]),
+    "holo_kv4_append": (_I, [_P, _I, _P, _P, _I, _I, _P]),
+    "holo_kv4_read": (_I, [_P, _I, _P, _P, _I, _I, _P]),
+    "holo_attention_kv4": (_I, [_P, _I, _P, _P, _I, _I, _I, _P]),
+    "holo_kv4_copy_pages": (_I, [_P, _P, _P, _I]),
+    "holo_kv4_pages_create": (_P, [_P]),
+    "holo_kv4_pages_destroy": (None, [_P]),
+    "holo_kv4_pages_reserve": (_I, [_P, _P, _P, _I]),
+    "holo_kv4_pages_fork": (_I, [_P, _P, _P, _I]),
+    "holo_kv4_pages_free": (_I, [_P, _P, _I]),
+    "holo_kv4_pages_compact": (_I, [_P]),
+    "holo_kv4_pages_available": (_I, [_P]),
+    "holo_kv4_pages_len": (_I, [_P, _I]),
+    "holo_kv4_pages_list": (_I, [_P, _I, _P, _I]),
 }
 
 _lib: C.CDLL | None = None
 
 
-EINVAL, ECHAIN = 100001, 100002
+EINVAL, ECHAIN, ENOPAGES = 100001, 100002, 100003
 
 
 class StreamStage(C.Structure):
@@ -284,6 +300,18 @@ class LlamaModel(C.Structure):
         ("rms_eps", C.c_float), ("rope_base", C.c_float), ("tok_emb", C.c_void_p), ("emb_type", C.c_int),
         ("out_norm", C.c_void_p), ("output", C.c_void_p), ("out_type", C.c_int), ("key_cache", C.c_void_p),
         ("value_cache", C.c_void_p), ("layers", C.POINTER(LlamaLayer))]
+
+
+class Batch(C.Structure):
+    """holo_batch_t (include/holo_forward.h)."""
+    _fields_ = [(n, C.c_int) for n in ("rows", "n_seqs", "max_rows", "max_len")] + [
+        ("cu_rows", C.c_void_p), ("seqs", C.c_void_p)]
+
+
+class KV4(C.Structure):
+    """holo_kv4_t (include/holo_forward.h)."""
+    _fields_ = [("pool", C.c_void_p), ("table", C.c_void_p), ("len", C.c_void_p)] + [
+        (n, C.c_int) for n in ("n_pages", "page_len", "n_layers", "n_kv_heads", "head_dim", "n_seqs", "max_pages")]
 
 
 class HoloError(RuntimeError):

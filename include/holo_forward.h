@@ -55,6 +55,114 @@ void holo_attention_prefill(float *out, const float *q, const float *k_cache, co
 void holo_matmul_rows(float *Y, const void *W, const float *X, int rows, int out_dim, int in_dim, int type,
                       int exact);
 
+/* ---- several sequences at once ------------------------------------------------
+ * A batch is the new rows of n_seqs sequences, packed: entry s has rows
+ * cu_rows[s] .. cu_rows[s + 1] - 1 (one in a decode step, a chunk or a whole
+ * prompt otherwise).  cu_rows and seqs are device arrays, so a captured graph
+ * follows what they hold at each replay; what they say past `rows` is cut off.
+ * rows, max_rows and max_len bound the launch: an entry's rows past its first
+ * max_rows are left as they were.  No rows or no entries: nothing is done.
+ * No reference counterpart (one sequence, one token at a time: llm.c:1015-1270). */
+typedef struct {
+    int rows;           /* rows of the call, over all entries */
+    int n_seqs;         /* entries, up to 65535 */
+    int max_rows;       /* the most rows of an entry */
+    int max_len;        /* holo_attention_kv4: the most positions of an entry's sequence */
+    const int *cu_rows; /* device, [n_seqs + 1], rising from 0 to rows */
+    const int *seqs;    /* device, [n_seqs]: the entry's sequence of the cache, each once; NULL: entry s is sequence s */
+} holo_batch_t;
+
+/* Causal attention within each sequence: row i of an entry against its rows 0
+ * .. i, softmax(q . k / sqrt(head_dim)) v, head h reading KV head h / (n_heads
+ * / n_kv_heads): the prompts of several sequences in one call
+ * (holo_attention_prefill at pos0 = 0, entry by entry).  ldo, ldq, ldk and ldv
+ * are the floats from one row to the next (q, k and v may lie side by side in
+ * one buffer).  head_dim 32, 64, 96 or 128; every pointer 16-byte aligned and
+ * every ld a multiple of 4.  seqs and max_len are not read.  A row is not
+ * touched by what the rows behind it hold, infinities and NaN among it.
+ * Returns 0 or HOLO_EINVAL (nothing launched).                               */
+int holo_attention_packed(float *out, const float *q, const float *k, const float *v, int ldo, int ldq, int ldk,
+                          int ldv, int head_dim, int n_heads, int n_kv_heads, const holo_batch_t *b);
+
+/* ---- a cache in pages, four bits a value -------------------------------------------
+ * Q4_0 values (16 codes about a block scale, 32 dims a block) in a layout for
+ * the matrix cores: a page holds page_len positions of every layer and KV head,
+ * in tiles of 32 positions of 36 * head_dim bytes (16 codes bytes a position and
+ * 32 dims for keys and for values each, and their f16 scales), 4.5 bits a value.
+ * A block's scale is d = -m / 8 of its value m of largest magnitude (the negative
+ * one of two), rounded to bfloat16, at most 2720 in magnitude and held in f16;
+ * a value is d * c, c the nearest to x / d in -8 .. 7 (ties to the even one).
+ * d has 8 significant bits, so d * c is an f16 and the products below are of
+ * exact operands.  A block that holds an infinity or NaN reads as NaN; values
+ * past 21760 are held as about that.
+ *
+ * pool, table and len are device memory of the caller.  Entry p of a sequence's
+ * row of `table` is the page of its positions p * page_len ..; an entry outside
+ * 0 .. n_pages - 1 is no page: nothing is stored there, and attention passes
+ * over its positions.  len holds each sequence's positions, the rows of the
+ * batch in hand among them: the last of them are the batch's.  Sequences may
+ * share pages (holo_kv4_pages_fork).                                           */
+typedef struct {
+    void *pool;       /* n_pages * holo_kv4_page_bytes bytes, 16-byte aligned */
+    const int *table; /* [n_seqs][max_pages] */
+    const int *len;   /* [n_seqs] */
+    int n_pages;
+    int page_len;     /* 32, 64, 128, 256, 512 or 1024 */
+    int n_layers, n_kv_heads;
+    int head_dim;     /* 32, 64, 96 or 128 */
+    int n_seqs, max_pages;
+} holo_kv4_t;
+
+/* Bytes of a page, or 0 for a layout outside the set above (only the layout is read). */
+size_t holo_kv4_page_bytes(const holo_kv4_t *c);
+/* The batch's rows of k and v ([n_kv_heads * head_dim] floats, ldk and ldv from
+ * one row to the next) into the pages of one layer, at the last positions of
+ * their sequences.  What the other positions hold stays.  0 or HOLO_EINVAL.     */
+int holo_kv4_append(const holo_kv4_t *c, int layer, const float *k, const float *v, int ldk, int ldv,
+                    const holo_batch_t *b);
+/* The values that the cache holds for the batch's rows (zeros where there is no page). */
+int holo_kv4_read(const holo_kv4_t *c, int layer, float *k, float *v, int ldk, int ldv, const holo_batch_t *b);
+/* Attention of the batch's rows over their sequences' pages: row i of an entry
+ * of r rows is at position len - r + i and sees the positions up to its own
+ * (cuda_multi_head_attention over several sequences, cuda_ops.h:112; with more
+ * rows holo_attention_prefill).  A row that sees no position gives zeros; the
+ * rows of a sequence longer than max_len give NaN.  q rows of n_heads *
+ * head_dim floats.  0 or HOLO_EINVAL; without memory for its partial sums the
+ * hipError_t.                                                                  */
+int holo_attention_kv4(const holo_kv4_t *c, int layer, float *out, const float *q, int ldo, int ldq, int n_heads,
+                       const holo_batch_t *b);
+/* Page dst[i] becomes a copy of page src[i], every layer (host arrays).
+ * HOLO_EINVAL, and nothing copied, for a page outside the pool, a page written
+ * twice, or one that is read and written.                                      */
+int holo_kv4_copy_pages(const holo_kv4_t *c, const int *src, const int *dst, int n);
+
+/* Which pages belong to which sequence, on the host: the lowest free page is
+ * taken first, and the device's table and len follow on the library stream.
+ * c's device arrays must outlive the handle and be written by it alone; a c
+ * without any (pool, table and len NULL) is bookkeeping without a device.  Calls
+ * return 0, HOLO_EINVAL (also under graph capture) or HOLO_ENOPAGES (reserve);
+ * then nothing has changed.  One handle may be used by several threads.        */
+typedef struct holo_kv4_pages holo_kv4_pages_t;
+/* Every sequence empty, every page free; NULL with the error latched.          */
+holo_kv4_pages_t *holo_kv4_pages_create(const holo_kv4_t *c);
+void holo_kv4_pages_destroy(holo_kv4_pages_t *p);
+/* Room for rows[i] more positions of sequence seqs[i] (host arrays, a sequence
+ * once), len counting them from now on: before a batch's append.  A sequence
+ * whose last page is not full and shared gets a copy of it.                    */
+int holo_kv4_pages_reserve(holo_kv4_pages_t *p, const int *seqs, const int *rows, int n);
+/* The empty sequence dst[i] becomes a copy of src[i], sharing its pages.  Entry
+ * by entry: a src may be an earlier dst.                                       */
+int holo_kv4_pages_fork(holo_kv4_pages_t *p, const int *src, const int *dst, int n);
+/* Sequences emptied; pages that no other sequence shares are free again.       */
+int holo_kv4_pages_free(holo_kv4_pages_t *p, const int *seqs, int n);
+/* The pages in use moved to the front of the pool: 0 .. used - 1.              */
+int holo_kv4_pages_compact(holo_kv4_pages_t *p);
+/* Pages free; positions of a sequence (-1: none such); its pages, at most n of
+ * them (host array), and how many it has.                                      */
+int holo_kv4_pages_available(holo_kv4_pages_t *p);
+int holo_kv4_pages_len(holo_kv4_pages_t *p, int seq);
+int holo_kv4_pages_list(holo_kv4_pages_t *p, int seq, int *pages, int n);
+
 /* ---- the model --------------------------------------------------------------- */
 
 typedef struct {

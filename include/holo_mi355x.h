@@ -28,6 +28,7 @@ extern "C" {
  * argument.  holo_last_error() returns and clears the latch.               */
 #define HOLO_EINVAL 100001
 #define HOLO_ECHAIN 100002  /* a persistent decode-step launch could not synchronise */
+#define HOLO_ENOPAGES 100003  /* not enough free pages in a cache (holo_forward.h) */
 int holo_last_error(void);
 const char *holo_error_string(int code);
 
