@@ -12,7 +12,7 @@
 //     c + 8, and one packed fma with d and -24 d makes d * c of it.
 //   - q (scaled by a power of two to its row's largest value) and the
 //     probabilities are two f16 halves, x - hi - lo within 2^-22 |x|: fp32's
-//     class with two matrix instructions.  Probabilities are held times 2^8, so
+//     class with two matrix instructions.  Probabilities are held times 2^7.5, so
 //     that a small one's lo stays above f16's smallest step.
 //   - The softmax is one pass: the running maximum of a column moves only when a
 //     score passes it by 2^7 (p then stays below 2^15), which few tiles do.
@@ -133,7 +133,10 @@ __global__ __launch_bounds__(64 * W) void attn_kv4_k(Kv4Attn a)
             x[j][0] = u.x, x[j][1] = u.y, x[j][2] = u.z, x[j][3] = u.w;
             x[j][4] = w.x, x[j][5] = w.y, x[j][6] = w.z, x[j][7] = w.w;
 #pragma unroll
-            for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[j][i]));
+            for (int i = 0; i < 8; i++) {
+                x[j][i] *= score_scale(HD);
+                big = fmaxf(big, fabsf(x[j][i]));
+            }
         }
         big = fmaxf(big, __shfl_xor(big, 16, 64));
         big = fmaxf(big, __shfl_xor(big, 32, 64));
@@ -145,7 +148,7 @@ __global__ __launch_bounds__(64 * W) void attn_kv4_k(Kv4Attn a)
             for (int i = 0; i < 8; i++) x[j][i] = ldexpf(x[j][i], -ex);
             split8(x[j], qh[j], ql[j]);
         }
-        sc = ldexpf(1.4426950408889634f / sqrtf((float)HD), ex);
+        sc = ldexpf(1.f, ex);
     }
 
     float m = -FLT_MAX, l = 0.f;  // of log2 units; l: this lane's positions

@@ -1,259 +1,362 @@
 // attn_packed.hip -- causal attention over packed sequences (holo_attention_packed).
 //
 // softmax(q . k_p / sqrt(hd)) . v_p over the rows p of the same sequence up to a
-// row's own.  Both products run on v_mfma_f32_16x16x32_f16, transposed (S^T = K
-// Q^T, O^T = V^T P^T), a lane holding one column (a row and query head); every
-// operand is two f16 halves, hi hi + hi lo + lo hi in fp32: x - hi - lo within
-// 2^-22 |x|.  q rows, and tiles of 32 keys and values, are scaled by a power of
-// two to their largest value first, so that no value is too large or small for
-// f16.
-//
-// A tile that holds an infinity or NaN is multiplied in fp32, value by value:
-// the matrix instructions would hand it to the rows that do not see it.
+// row's own.  Both products run on v_mfma_f32_32x32x16_f16, transposed (S^T = K
+// Q^T, O^T = V^T P^T): lane j + 32 hh holds column j (a row and query head) of its
+// wave's 32 throughout, the scores of keys (r % 4) + 8 (r / 4) + 4 hh in
+// registers r < 16.  Every operand is two f16 halves, hi hi + hi lo + lo hi in
+// fp32 (x - hi - lo within 2^-22 |x|).
+//   - A workgroup's four waves take 128 columns (rows times the query heads that
+//     share a KV head) and walk the keys together, 32 at a time: a tile is split
+//     into halves once, into LDS, and read by all four as the operands they need.
+//     Two tiles are in LDS and a third's loads under way.
+//   - LDS holds operands in the lanes' order, 16 bytes a lane.  V is turned on the
+//     way in: a thread loads four dims of the eight keys that make up a register
+//     group of the scores, so that the probabilities are the second product's B
+//     operand where they stand.  Pieces are permuted (XOR) so that both the
+//     writes and the reads of 16 lanes fall on 64 different banks.
+//   - Keys and values are held times 2^8, which suits f16 for rows whose largest
+//     value is in [2^-11, 2^8); q rows are scaled to their largest value.  Where
+//     the keys that a workgroup walks hold any other row (or an infinity or NaN,
+//     which the matrix instructions would hand to the rows that do not see it), it
+//     starts over in fp32, value by value: right for anything, and slow.
+//   - The softmax is one pass; the running maximum moves only when a score passes
+//     it by 2^7 (attn_tiles.h).
+// KV heads are the fastest grid index, so that with 8 of them each XCD's L2 holds
+// one head's keys and values.
 #include "attn_tiles.h"
 #include "kv4.h"
 
 namespace holo {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
 struct PackedAttn {
     holo_batch_t b;
     float *out;
     const float *q, *k, *v;
     int ldo, ldq, ldk, ldv, n_heads, n_kv_heads;
-    int ctiles;  // tiles of 16 columns that max_rows rows have
 };
 
-// The exponent that brings a largest value to [2^13, 2^14).
-__device__ __forceinline__ int scale_exp(float big) { return big > 0.f ? ilogbf(big) - 13 : -4000; }
+constexpr float kHeld = 256.f;                               // keys and values are held times this
+constexpr float kRowLow = 1.f / 2048.f, kRowHigh = 256.f;    // a row's largest value
 
-template <int NB, int W>
-__global__ __launch_bounds__(64 * W) void attn_packed_k(PackedAttn a)
+// x * kHeld = hi + lo.
+__device__ __forceinline__ void split_held(float x, _Float16 &hi, _Float16 &lo)
 {
-    constexpr int HD = 32 * NB, OS = HD + 4;
-    __shared__ __align__(16) float lo_[W][16][OS];
-    __shared__ float lm[W][16], ll[W][16];
-    __shared__ int le[W];
+    hi = (_Float16)(x * kHeld);
+    lo = (_Float16)fmaf(x, kHeld, -(float)hi);
+}
+
+// The largest magnitude of four values; NaN if one is.
+__device__ __forceinline__ float most(const f4 x)
+{
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(x.x), fabsf(x.y)),
+                                         __builtin_elementwise_maximum(fabsf(x.z), fabsf(x.w)));
+}
+
+// Whether a row of LPR lanes, in any of the wave's 64 / LPR, has a largest value
+// that is not 0 and below kRowLow.
+template <int LPR>
+__device__ __forceinline__ bool low_row(float m)
+{
+    const unsigned long long ge = __ballot(m >= kRowLow);
+    constexpr unsigned long long one = LPR == 32 ? 0xFFFFFFFFull : LPR == 16 ? 0xFFFFull : 0xFFull;
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < 64 / LPR; i++) all &= (ge >> (LPR * i) & one) != 0;
+    if (all) return false;
+    const unsigned long long pos = __ballot(m > 0.f);
+    bool low = false;
+#pragma unroll
+    for (int i = 0; i < 64 / LPR; i++) low |= (pos >> (LPR * i) & one) != 0 && (ge >> (LPR * i) & one) == 0;
+    return low;
+}
+
+template <int NB>
+struct PackedLds {
+    static constexpr int HD = 32 * NB;  // HD / 8 <= 16
+    // [hi, lo][dims 8 d8 ..][key ^ (d8 & 15)] and [hi, lo][dims 32 b ..][keys' group][dim]
+    h8 k[2][2][HD / 8][32], v[2][2][NB][4][32];
+    int odd[2][2][4];  // by half and staging wave: a row that the halves do not suit
+};
+
+// One column in fp32 by the two lanes that hold it, half of the dims each.
+template <int HD>
+__device__ __forceinline__ void packed_fp32(const PackedAttn &a, const float *qp, const float *kb, const float *vb,
+                                            int row, int hh, float *out)
+{
+#pragma clang fp contract(off)  // the largest score less itself has to be 0
+    constexpr int H = HD / 2;
+    float m = -FLT_MAX, l = 0.f;
+    f4 o[H / 4];
+#pragma unroll
+    for (int i = 0; i < H / 4; i++) o[i] = f4{};
+    qp += H * hh, kb += H * hh, vb += H * hh, out += H * hh;
+    for (int key = 0; key <= row; key++) {
+        const f4 *k = (const f4 *)(kb + (int64_t)key * a.ldk), *v = (const f4 *)(vb + (int64_t)key * a.ldv);
+        f4 d4 = f4{};
+#pragma unroll 4
+        for (int i = 0; i < H / 4; i++) d4 += ((const f4 *)qp)[i] * k[i];
+        float s = (d4[0] + d4[1]) + (d4[2] + d4[3]);
+        s = (s + __shfl_xor(s, 32, 64)) * score_scale(HD);
+        const float mx = fmaxf(m, s), w = __builtin_amdgcn_exp2f(m - mx), p = __builtin_amdgcn_exp2f(s - mx);
+        m = mx;
+        // the average so far: a sum of values next to the largest float would overflow
+        const float was = l * w;
+        l = was + p;
+        const float keep = was / l, add = p / l;
+#pragma unroll
+        for (int i = 0; i < H / 4; i++) o[i] = o[i] * keep + add * v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < H / 4; i++) ((f4 *)out)[i] = o[i];
+}
+
+template <int NB>
+__global__ __launch_bounds__(256, 2) void attn_packed_k(PackedAttn a)
+{
+    constexpr int HD = 32 * NB, NC = HD / 16, D4 = HD / 4;
+    constexpr int LPR = HD == 32 ? 8 : HD == 64 ? 16 : 32;  // lanes of a row (HD 96: the last eight idle)
+    constexpr int VW = NB > 2 ? 2 : 1;                       // waves that stage V, the others K
+    extern __shared__ __align__(16) uint8_t packed_lds[];
+    PackedLds<NB> &S = *(PackedLds<NB> *)packed_lds;
     const int G = a.n_heads / a.n_kv_heads;
-    const int kvh = blockIdx.y, ct = gridDim.x - 1 - blockIdx.x;  // the longest first
+    const int kvh = blockIdx.x, ct = gridDim.y - 1 - blockIdx.y;  // the longest first
     const int s0 = min(max(a.b.cu_rows[blockIdx.z], 0), a.b.rows);
     const int n = min(min(max(a.b.cu_rows[blockIdx.z + 1], s0), a.b.rows) - s0, a.b.max_rows);
-    const int ncols = n * G, c0 = 16 * ct;
+    const int ncols = n * G, c0 = 128 * ct;
     if (c0 >= ncols) return;
-    const int last_row = (min(c0 + 16, ncols) - 1) / G, first_row = c0 / G;
-    const int ntiles = (last_row + 32) >> 5;
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int col = c0 + r;
-    const bool valid = col < ncols;
-    const int row = valid ? col / G : first_row, head = kvh * G + (valid ? col % G : 0);
+    const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ntiles = ((min(c0 + 128, ncols) - 1) / G + 32) >> 5;
+    // the wave's columns, from row w_first on
+    const int w0 = c0 + 32 * wave;
+    const int w_first = w0 / G;
+    const int col = min(w0 + j, ncols - 1);
+    const int row = col / G, head = kvh * G + col % G;
     const float *qp = a.q + (int64_t)(s0 + row) * a.ldq + (int64_t)head * HD;
     const float *kb = a.k + (int64_t)s0 * a.ldk + (int64_t)kvh * HD;
     const float *vb = a.v + (int64_t)s0 * a.ldv + (int64_t)kvh * HD;
 
-    h8 qh[NB], ql[NB];
-    float sc;
-    {
-        float x[NB][8], big = 0.f;
+    // ---- staging: a tile's pieces from memory to registers, and into LDS.  Buffer
+    // loads from the tile's first row: rows past the sequence, and the idle lanes
+    // of HD 96, read zeros.
+    f4 ld[4];
+    const bool stages_v = wave < VW;
+    const int x4 = lane % LPR;  // the thread's four dims
+    const bool on = HD != 96 || x4 < D4;
+    // V: group vg of eight keys (register group vg / 2, half vg % 2): 4 (vg & 1) + 16 (vg >> 1) + 0..3 and + 8..11;
+    // K: row kr and every KS-th, KH of them a half
+    constexpr int KS = 64 * (4 - VW) / LPR, KH = (32 + 2 * KS - 1) / (2 * KS);
+    const int vg = tid / LPR, kr = (tid - 64 * VW) / LPR;
+    const float *xb = stages_v ? vb : kb;
+    const uint32_t rowb = 4u * (uint32_t)(stages_v ? a.ldv : a.ldk);
+    const bool mine = on && (!stages_v || vg < 4);
+    const uint32_t vo = mine ? (uint32_t)(stages_v ? 16 * (vg >> 1) + 4 * (vg & 1) : kr) * rowb + 16u * x4 : 0x80000000u;
+    // Half f of a tile: a thread's first or last four keys of V, or its first or
+    // last pieces of K (a whole tile in registers spilled, HD 128).
+    auto load = [&](int t, int f) {
+        const int rows = min(n - 32 * t, 32);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)(xb + (int64_t)32 * t * (rowb >> 2)), (short)0, (int)((uint32_t)(rows - 1) * rowb + 4u * HD),
+            kRawBufWord3);
 #pragma unroll
-        for (int j = 0; j < NB; j++) {
-            const float4 u = *(const float4 *)(qp + 8 * (NB * g + j)), w = *(const float4 *)(qp + 8 * (NB * g + j) + 4);
-            x[j][0] = u.x, x[j][1] = u.y, x[j][2] = u.z, x[j][3] = u.w;
-            x[j][4] = w.x, x[j][5] = w.y, x[j][6] = w.z, x[j][7] = w.w;
-#pragma unroll
-            for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[j][i]));
+        for (int i = 0; i < 4; i++) {
+            if (!stages_v && i >= KH) continue;
+            const uint32_t r = stages_v ? i + 8 * f : KS * (KH * f + i);
+            ld[i] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)vo, (int)(r * rowb), 0));
         }
-        big = fmaxf(big, __shfl_xor(big, 16, 64));
-        big = fmaxf(big, __shfl_xor(big, 32, 64));
-        const int ex = big > 0.f && big <= FLT_MAX ? scale_exp(big) : 0;
+    };
+    auto store = [&](int b, int f) {
+        bool odd = false;
+        float big = 0.f;
+        if (stages_v) {
+            h4 hi[4], lo[4];
 #pragma unroll
-        for (int j = 0; j < NB; j++) {
+            for (int i = 0; i < 4; i++) {
+                const float m = most(ld[i]);
+                big = __builtin_elementwise_maximum(big, m);
+                odd |= low_row<LPR>(m);
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[j][i] = ldexpf(x[j][i], -ex);
-            split8(x[j], qh[j], ql[j]);
-        }
-        sc = ldexpf(1.4426950408889634f / sqrtf((float)HD), ex);
-    }
-
-    float m = -FLT_MAX, l = 0.f;
-    int E = -4000;  // the outputs are held times 2^-E
-    f4 o[2 * NB];
-#pragma unroll
-    for (int i = 0; i < 2 * NB; i++) o[i] = f4{};
-
-    for (int t = wave; t < ntiles; t += W) {
-        const int p0 = 32 * t;
-        // keys: rows p0 + 16 h + r (past the sequence: its last row, not seen)
-        float kx[2][NB][8], big = 0.f;
-        bool bad = false;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int pos = min(p0 + 16 * h + r, n - 1);
-            const float *kp = kb + (int64_t)pos * a.ldk + 8 * NB * g;
-#pragma unroll
-            for (int j = 0; j < NB; j++) {
-                const float4 u = *(const float4 *)(kp + 8 * j), w = *(const float4 *)(kp + 8 * j + 4);
-                float *x = kx[h][j];
-                x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    bad |= !(fabsf(x[i]) <= FLT_MAX);
-                    big = fmaxf(big, fabsf(x[i]));
+                for (int d = 0; d < 4; d++) {
+                    _Float16 h, l;
+                    split_held(ld[i][d], h, l);
+                    hi[d][i] = h;
+                    lo[d][i] = l;
                 }
             }
-        }
-        float p[8];
-        if (__any(bad)) {
-            for (int i = 0; i < 8; i++) {
-                const int pos = p0 + v_pos(g, i);
-                float d = 0.f;
-                if (pos <= row)
-                    for (int j = 0; j < HD; j++) d = fmaf(qp[j], kb[(int64_t)pos * a.ldk + j], d);
-                p[i] = d * (1.4426950408889634f / sqrtf((float)HD));
+            if (mine) {
+                const int vb_ = x4 >> 3, at = 4 * (x4 & 7), sw = (x4 >> 2 & 1) + 2 * (vb_ & 1);
+#pragma unroll
+                for (int d = 0; d < 4; d++) {
+                    ((h4 *)&S.v[b][0][vb_][vg][at + (d ^ sw)])[f] = hi[d];
+                    ((h4 *)&S.v[b][1][vb_][vg][at + (d ^ sw)])[f] = lo[d];
+                }
             }
         } else {
 #pragma unroll
-            for (int x = 1; x < 64; x <<= 1) big = fmaxf(big, __shfl_xor(big, x, 64));
-            const int ek = big > 0.f ? scale_exp(big) : 0;
-            f4 s[2] = {f4{}, f4{}};
+            for (int i = 0; i < KH; i++) {
+                const int r = kr + KS * (KH * f + i);
+                const float m = most(ld[i]);
+                big = __builtin_elementwise_maximum(big, m);
+                odd |= low_row<LPR>(m);
+                h4 hi, lo;
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int j = 0; j < NB; j++) {
-                    h8 kh, kl;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) kx[h][j][i] = ldexpf(kx[h][j][i], -ek);
-                    split8(kx[h][j], kh, kl);
-                    s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[j], s[h], 0, 0, 0);
-                    s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[j], s[h], 0, 0, 0);
-                    s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[j], s[h], 0, 0, 0);
+                for (int d = 0; d < 4; d++) {
+                    _Float16 h, l;
+                    split_held(ld[i][d], h, l);
+                    hi[d] = h;
+                    lo[d] = l;
                 }
-#pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = ldexpf(s[i >> 2][i & 3] * sc, ek);
+                if (mine && (2 * KH * KS == 32 || r < 32)) {
+                    const int d8 = x4 >> 1;
+                    ((h4 *)&S.k[b][0][d8][r ^ (d8 & 15)])[x4 & 1] = hi;
+                    ((h4 *)&S.k[b][1][d8][r ^ (d8 & 15)])[x4 & 1] = lo;
+                }
+            }
         }
+        odd |= __any(!(big < kRowHigh));
+        if (lane == 0) S.odd[b][f][wave] = odd;
+    };
+    load(0, 0);
+
+    h8 qh[NC], ql[NC];
+    float sc;
+    {
+        float x[NC][8], big = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (p0 + v_pos(g, i) > row) p[i] = -INFINITY;
-        float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+        for (int c = 0; c < NC; c++) {
+            const float4 u = *(const float4 *)(qp + 16 * c + 8 * hh), w = *(const float4 *)(qp + 16 * c + 8 * hh + 4);
+            x[c][0] = u.x, x[c][1] = u.y, x[c][2] = u.z, x[c][3] = u.w;
+            x[c][4] = w.x, x[c][5] = w.y, x[c][6] = w.z, x[c][7] = w.w;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[c][i] *= score_scale(HD);
+                big = fmaxf(big, fabsf(x[c][i]));
+            }
+        }
+        big = fmaxf(big, __shfl_xor(big, 32, 64));
+        // to [2^13, 2^14); rows of zeros, and rows with an infinity (whose halves make NaN of it), as they are
+        const int ex = big > 0.f && big <= FLT_MAX ? ilogbf(big) - 13 : 0;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[c][i] = ldexpf(x[c][i], -ex);
+            split8(x[c], qh[c], ql[c]);
+        }
+        sc = ldexpf(1.f / kHeld, ex);
+    }
+    store(0, 0);
+    load(0, 1);
+    store(0, 1);
+    __syncthreads();
+
+    float m = -FLT_MAX, l = 0.f;
+    f16v o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) o[i] = f16v{};
+
+    // the probabilities of a tile's scores, and their values
+    auto values = [&](int b, f16v s) {
+        float ps[4] = {};
+        const float off = kPShift - m;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, off));
+            ps[r & 3] += s[r];
+        }
+        l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            const float p8[8] = {s[8 * ks],     s[8 * ks + 1], s[8 * ks + 2], s[8 * ks + 3],
+                                 s[8 * ks + 4], s[8 * ks + 5], s[8 * ks + 6], s[8 * ks + 7]};
+            h8 ph, pl;
+            split8(p8, ph, pl);
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                const int at = j ^ ((j >> 4 & 1) + 2 * (i & 1));
+                const h8 vh = S.v[b][0][i][2 * ks + hh][at], vl = S.v[b][1][i][2 * ks + hh][at];
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph, o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl, o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, o[i], 0, 0, 0);
+            }
+        }
+    };
+    bool over = false;  // a tile that the halves do not suit
+    for (int t = 0; t < ntiles; t++) {
+        const int b = t & 1, key0 = 32 * t;
+        const int4 odd0 = *(const int4 *)S.odd[b][0], odd1 = *(const int4 *)S.odd[b][1];
+        over = __builtin_amdgcn_readfirstlane(odd0.x | odd0.y | odd0.z | odd0.w | odd1.x | odd1.y | odd1.z | odd1.w);
+        if (over) break;
+        const bool more = t + 1 < ntiles;
+        if (more) load(t + 1, 0);
+        f16v s = f16v{};
+        int jh = j ^ hh;  // (opaque: a step's address is one XOR, not a register kept for it)
+        asm volatile("" : "+v"(jh));
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const h8 kh = S.k[b][0][2 * c + hh][jh ^ (2 * c)], kl = S.k[b][1][2 * c + hh][jh ^ (2 * c)];
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[c], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[c], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[c], s, 0, 0, 0);
+        }
+        if (key0 + 31 > w_first) {
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (key0 + (r & 3) + 8 * (r >> 2) + 4 * hh > row) s[r] = -INFINITY;
+        }
+        if (more) {
+            store(b ^ 1, 0);  // last read a tile ago, before the barrier
+            load(t + 1, 1);
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[r]);
+        mx *= sc;
+        // two forms of the rest: a scaling of the outputs that only some tiles need
+        // made the compiler copy them every tile
         if (__any(mx > m + kMaxSlack)) {
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
             const float w = __builtin_amdgcn_exp2f(m - mx);
             m = mx;
             l *= w;
 #pragma unroll
-            for (int i = 0; i < 2 * NB; i++) o[i] *= w;
+            for (int i = 0; i < NB; i++) o[i] *= w;
+            values(b, s);
+        } else {
+            values(b, s);
         }
-        float ps = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            p[i] = __builtin_amdgcn_exp2f(p[i] - m + kPShift);
-            ps += p[i];
-        }
-        l += ps;
-        // values: dim 16 i + r of the lane's eight positions
-        float vx[2 * NB][8];
-        big = 0.f;
-        bad = false;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int pos = p0 + v_pos(g, j);
-            const bool in = pos <= last_row;
-            const float *vp = vb + (int64_t)min(pos, last_row) * a.ldv + r;
-#pragma unroll
-            for (int i = 0; i < 2 * NB; i++) {
-                const float y = in ? vp[16 * i] : 0.f;
-                vx[i][j] = y;
-                bad |= !(fabsf(y) <= FLT_MAX);
-                big = fmaxf(big, fabsf(y));
-            }
-        }
-        if (__any(bad)) {
-            if (E < -2000) E = 0;
-            for (int x = 0; x <= last_row - p0 && x < 32; x++) {
-                // x's probability: value 4 (x / 16) + x % 4 of lane group (x / 4) % 4
-                float w = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (i == 4 * (x >> 4) + (x & 3)) w = p[i];
-                w = __shfl(w, ((x >> 2) & 3) * 16 + r, 64);
-                if (p0 + x > row) continue;
-                const float *vp = vb + (int64_t)(p0 + x) * a.ldv + 4 * g;
-#pragma unroll
-                for (int i = 0; i < 2 * NB; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) o[i][j] = fmaf(w, ldexpf(vp[16 * i + j], -E), o[i][j]);
-            }
-            continue;
-        }
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) big = fmaxf(big, __shfl_xor(big, x, 64));
-        const int ev = scale_exp(big);
-        if (ev <= -4000) continue;  // values of zero
-        if (ev > E) {
-#pragma unroll
-            for (int i = 0; i < 2 * NB; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) o[i][j] = ldexpf(o[i][j], E - ev);
-            E = ev;
-        }
-        h8 ph, pl;
-#pragma unroll
-        for (int i = 0; i < 8; i++) p[i] = ldexpf(p[i], ev - E);
-        split8(p, ph, pl);
-#pragma unroll
-        for (int i = 0; i < 2 * NB; i++) {
-            h8 vh, vl;
-#pragma unroll
-            for (int j = 0; j < 8; j++) vx[i][j] = ldexpf(vx[i][j], -ev);
-            split8(vx[i], vh, vl);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[i], 0, 0, 0);
-        }
+        if (more) store(b ^ 1, 1);
+        __syncthreads();
     }
-
-    // the waves meet: O = sum_w 2^(m_w - M + E_w) O_w
-    l += __shfl_xor(l, 16, 64);
+    if (over) {
+        if (w0 + j < ncols) packed_fp32<HD>(a, qp, kb, vb, row, hh, a.out + (int64_t)(s0 + row) * a.ldo + (int64_t)head * HD);
+        return;
+    }
     l += __shfl_xor(l, 32, 64);
+    if (w0 + j >= ncols) return;
+    const float f = 1.0f / (kHeld * l);  // a row sees itself
+    float *op = a.out + (int64_t)(s0 + row) * a.ldo + (int64_t)head * HD + 4 * hh;
 #pragma unroll
-    for (int i = 0; i < 2 * NB; i++) *(f4 *)&lo_[wave][r][16 * i + 4 * g] = o[i];
-    if (g == 0) {
-        lm[wave][r] = m;
-        ll[wave][r] = l;
-    }
-    if (lane == 0) le[wave] = E;
-    __syncthreads();
-    int top = le[0];
+    for (int i = 0; i < NB; i++)
 #pragma unroll
-    for (int w = 1; w < W; w++) top = max(top, le[w]);
-    for (int i = threadIdx.x; i < 16 * (HD / 4); i += 64 * W) {
-        const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
-        if (c0 + c >= ncols) continue;
-        float M = lm[0][c];
-#pragma unroll
-        for (int w = 1; w < W; w++) M = fmaxf(M, lm[w][c]);
-        float L = 0.f;
-        f4 O = f4{};
-#pragma unroll
-        for (int w = 0; w < W; w++) {
-            const float f = __builtin_amdgcn_exp2f(lm[w][c] - M);
-            L = fmaf(f, ll[w][c], L);
-            O += ldexpf(f, le[w] - top) * *(const f4 *)&lo_[w][c][d];
-        }
-        const float f = 1.0f / L;  // a row sees itself
-        f4 y = O * f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) y[j] = ldexpf(y[j], top);
-        const int h = kvh * G + (c0 + c) % G;
-        *(f4 *)(a.out + (int64_t)(s0 + (c0 + c) / G) * a.ldo + (int64_t)h * HD + d) = y;
-    }
+        for (int r = 0; r < 16; r += 4)
+            *(f4 *)(op + 32 * i + 2 * r) = f4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]} * f;
 }
 
 template <int NB>
-static void run_packed(const PackedAttn &a)
+static void run_packed(const PackedAttn &a, int ctiles)
 {
-    constexpr int W = 4;
-    hipLaunchKernelGGL((attn_packed_k<NB, W>), dim3(a.ctiles, a.n_kv_heads, a.b.n_seqs), dim3(64 * W), 0, stream(), a);
+    constexpr size_t lds = sizeof(PackedLds<NB>);
+    static bool attr = false;
+    if (!attr) {
+        HOLO_CHECK(hipFuncSetAttribute((const void *)attn_packed_k<NB>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)lds));
+        attr = true;
+    }
+    hipLaunchKernelGGL(attn_packed_k<NB>, dim3(a.n_kv_heads, ctiles, a.b.n_seqs), dim3(256), lds, stream(), a);
     HOLO_LAUNCH_CHECK();
 }
 
@@ -272,20 +375,20 @@ extern "C" int holo_attention_packed(float *out, const float *q, const float *k,
     }
     if (b->rows == 0 || b->n_seqs == 0) return 0;
     const int64_t q_dim = (int64_t)n_heads * head_dim, kv_dim = (int64_t)n_kv_heads * head_dim;
-    PackedAttn a{*b, out, q, k, v, ldo, ldq, ldk, ldv, n_heads, n_kv_heads, 0};
+    PackedAttn a{*b, out, q, k, v, ldo, ldq, ldk, ldv, n_heads, n_kv_heads};
     a.b.max_rows = b->max_rows < b->rows ? b->max_rows : b->rows;
-    const int64_t cols = (int64_t)a.b.max_rows * (n_heads / n_kv_heads);
+    const int64_t ctiles = ((int64_t)a.b.max_rows * (n_heads / n_kv_heads) + 127) / 128;
+    const int most_ld = 1 << 24;  // 32 rows' bytes in 31 bits
     if (!rows_ok(out, ldo, q_dim) || !rows_ok(q, ldq, q_dim) || !rows_ok(k, ldk, kv_dim) || !rows_ok(v, ldv, kv_dim) ||
-        cols > 0x7FFFFF00) {
-        HOLO_REJECT("holo_attention_packed: null or misaligned rows, or rows that overlap");
+        ctiles > 65535 || ldk >= most_ld || ldv >= most_ld) {
+        HOLO_REJECT("holo_attention_packed: null or misaligned rows, rows that overlap, or more than one launch takes");
         return HOLO_EINVAL;
     }
-    a.ctiles = (int)((cols + 15) / 16);
     switch (head_dim) {
-    case 32: run_packed<1>(a); break;
-    case 64: run_packed<2>(a); break;
-    case 96: run_packed<3>(a); break;
-    default: run_packed<4>(a); break;
+    case 32: run_packed<1>(a, (int)ctiles); break;
+    case 64: run_packed<2>(a, (int)ctiles); break;
+    case 96: run_packed<3>(a, (int)ctiles); break;
+    default: run_packed<4>(a, (int)ctiles); break;
     }
     return 0;
 }

@@ -15,9 +15,18 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// Probabilities are held times 2^kPShift; a running maximum (log2 units) moves
-// when a score passes it by kMaxSlack.
-constexpr float kPShift = 8.f, kMaxSlack = 7.f;
+// Scores are in log2 units.  q is multiplied by this before it is split: what is
+// left to multiply a score by is a power of two, so that the largest one less
+// itself is 0 at any magnitude.
+constexpr float score_scale(int hd)
+{
+    return hd == 32 ? 0.25503486f : hd == 64 ? 0.18033688f : hd == 96 ? 0.14724444f : 0.12751743f;  // log2(e) / sqrt(hd)
+}
+
+// Probabilities are held times 2^kPShift; a running maximum moves when a score
+// passes it by kMaxSlack: they stay below 2^15.  (7.5: where 8 is half of the
+// maximum's last place, the sum of the two could round to 16.)
+constexpr float kPShift = 7.5f, kMaxSlack = 7.f;
 
 // x = hi + lo, two values at a time (x - hi is exact in fp32).
 __device__ __forceinline__ void split8(const float x[8], h8 &hi, h8 &lo)

@@ -130,6 +130,22 @@ def test_rows_behind_do_not_reach_a_row(holo):
         assert normwise(second[ok], w2[ok]) <= TOL
 
 
+def test_large_rows_behind_do_not_take_a_rows_precision(holo):
+    print("case packed wide range", flush=True)
+    hd, heads, n_kv, rows = 64, 4, 2, [100]
+    q, k, v = inputs(7, 100, hd, heads, n_kv)
+    want = want_packed(q, k, v, rows, hd, heads, n_kv)
+    for at in (20, 45, 70):
+        k2, v2 = k.copy(), v.copy()
+        k2[at] *= np.float32(1e25)
+        v2[at] *= np.float32(1e30)
+        got = run(holo, q, k2, v2, rows, hd, heads, n_kv)
+        assert normwise(got[:at], want[:at]) <= TOL
+        want2 = want_packed(q, k2, v2, rows, hd, heads, n_kv)
+        for i in range(at, 100):
+            assert normwise(got[i], want2[i]) <= TOL
+
+
 def test_captured(holo):
     """A captured call follows the device's cu_rows at each replay."""
     print("case packed graph", flush=True)
