@@ -258,8 +258,16 @@ __global__ __launch_bounds__(256, 2) void attn_packed_k(PackedAttn a)
 #pragma unroll
     for (int i = 0; i < NB; i++) o[i] = f16v{};
 
+    // operand x of a tile's values: dims 32 (x % NB) .., keys 16 (x / NB) ..
+    h8 vh, vl;
+    auto read_v = [&](int b, int x) {
+        const int i = x % NB, at = j ^ ((j >> 4 & 1) + 2 * (i & 1)), g = 2 * (x / NB) + hh;
+        vh = S.v[b][0][i][g][at];
+        vl = S.v[b][1][i][g][at];
+    };
     // the probabilities of a tile's scores, and their values
     auto values = [&](int b, f16v s) {
+        read_v(b, 0);
         float ps[4] = {};
         const float off = kPShift - m;
 #pragma unroll
@@ -268,68 +276,92 @@ __global__ __launch_bounds__(256, 2) void attn_packed_k(PackedAttn a)
             ps[r & 3] += s[r];
         }
         l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        h8 ph[2], pl[2];
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
             const float p8[8] = {s[8 * ks],     s[8 * ks + 1], s[8 * ks + 2], s[8 * ks + 3],
                                  s[8 * ks + 4], s[8 * ks + 5], s[8 * ks + 6], s[8 * ks + 7]};
-            h8 ph, pl;
-            split8(p8, ph, pl);
+            split8(p8, ph[ks], pl[ks]);
+        }
 #pragma unroll
-            for (int i = 0; i < NB; i++) {
-                const int at = j ^ ((j >> 4 & 1) + 2 * (i & 1));
-                const h8 vh = S.v[b][0][i][2 * ks + hh][at], vl = S.v[b][1][i][2 * ks + hh][at];
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph, o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl, o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, o[i], 0, 0, 0);
-            }
+        for (int x = 0; x < 2 * NB; x++) {
+            const int i = x % NB, ks = x / NB;
+            const h8 h = vh, l = vl;
+            if (x + 1 < 2 * NB) read_v(b, x + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h, ph[ks], o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h, pl[ks], o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l, ph[ks], o[i], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
+    auto rest = [&](int t) {  // of a tile: the second half of the next one into LDS
+        if (t + 1 < ntiles) store((t + 1) & 1, 1);
+        __syncthreads();
+    };
     bool over = false;  // a tile that the halves do not suit
-    for (int t = 0; t < ntiles; t++) {
-        const int b = t & 1, key0 = 32 * t;
-        const int4 odd0 = *(const int4 *)S.odd[b][0], odd1 = *(const int4 *)S.odd[b][1];
-        over = __builtin_amdgcn_readfirstlane(odd0.x | odd0.y | odd0.z | odd0.w | odd1.x | odd1.y | odd1.z | odd1.w);
-        if (over) break;
-        const bool more = t + 1 < ntiles;
-        if (more) load(t + 1, 0);
-        f16v s = f16v{};
-        int jh = j ^ hh;  // (opaque: a step's address is one XOR, not a register kept for it)
-        asm volatile("" : "+v"(jh));
+    int t = 0;
+    for (;;) {
+        f16v s;
+        bool moves = false;  // the running maximum, at tile t
+        // Tiles that leave the maximum alone, in a loop of their own: with the
+        // scaling of the outputs in it the compiler copied them every tile.
+        for (; t < ntiles; t++) {
+            const int b = t & 1, key0 = 32 * t;
+            const int4 odd0 = *(const int4 *)S.odd[b][0], odd1 = *(const int4 *)S.odd[b][1];
+            over = __builtin_amdgcn_readfirstlane(odd0.x | odd0.y | odd0.z | odd0.w | odd1.x | odd1.y | odd1.z | odd1.w);
+            if (over) break;
+            const bool more = t + 1 < ntiles;
+            if (more) load(t + 1, 0);
+            s = f16v{};
+            // (opaque: a step's address is one XOR, not a register kept for it)
+            int jh = j ^ hh;
+            asm volatile("" : "+v"(jh));
+            // a step's operands are read under the step before
+            h8 kh = S.k[b][0][hh][jh], kl = S.k[b][1][hh][jh];
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const h8 kh = S.k[b][0][2 * c + hh][jh ^ (2 * c)], kl = S.k[b][1][2 * c + hh][jh ^ (2 * c)];
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[c], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[c], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[c], s, 0, 0, 0);
-        }
-        if (key0 + 31 > w_first) {
+            for (int c = 0; c < NC; c++) {
+                const h8 h = kh, l = kl;
+                if (c + 1 < NC) {
+                    const int d8 = 2 * (c + 1);
+                    kh = S.k[b][0][d8 + hh][jh ^ d8];
+                    kl = S.k[b][1][d8 + hh][jh ^ d8];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(h, qh[c], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(h, ql[c], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(l, qh[c], s, 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (key0 + 31 > w_first) {
 #pragma unroll
-            for (int r = 0; r < 16; r++)
-                if (key0 + (r & 3) + 8 * (r >> 2) + 4 * hh > row) s[r] = -INFINITY;
+                for (int r = 0; r < 16; r++)
+                    if (key0 + (r & 3) + 8 * (r >> 2) + 4 * hh > row) s[r] = -INFINITY;
+            }
+            if (more) {
+                store(b ^ 1, 0);  // last read a tile ago, before the barrier
+                load(t + 1, 1);
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[r]);
+            moves = __any(mx * sc > m + kMaxSlack);
+            if (moves) break;
+            values(b, s);
+            rest(t);
         }
-        if (more) {
-            store(b ^ 1, 0);  // last read a tile ago, before the barrier
-            load(t + 1, 1);
-        }
+        if (!moves || over) break;
         float mx = s[0];
 #pragma unroll
         for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[r]);
-        mx *= sc;
-        // two forms of the rest: a scaling of the outputs that only some tiles need
-        // made the compiler copy them every tile
-        if (__any(mx > m + kMaxSlack)) {
-            mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
-            const float w = __builtin_amdgcn_exp2f(m - mx);
-            m = mx;
-            l *= w;
+        mx = fmaxf(m, sc * fmaxf(mx, __shfl_xor(mx, 32, 64)));
+        const float w = __builtin_amdgcn_exp2f(m - mx);
+        m = mx;
+        l *= w;
 #pragma unroll
-            for (int i = 0; i < NB; i++) o[i] *= w;
-            values(b, s);
-        } else {
-            values(b, s);
-        }
-        if (more) store(b ^ 1, 1);
-        __syncthreads();
+        for (int i = 0; i < NB; i++) o[i] *= w;
+        values(t & 1, s);
+        rest(t++);
     }
     if (over) {
         if (w0 + j < ncols) packed_fp32<HD>(a, qp, kb, vb, row, hh, a.out + (int64_t)(s0 + row) * a.ldo + (int64_t)head * HD);
