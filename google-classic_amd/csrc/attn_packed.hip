@@ -42,13 +42,6 @@ struct PackedAttn {
 constexpr float kHeld = 256.f;                               // keys and values are held times this
 constexpr float kRowLow = 1.f / 2048.f, kRowHigh = 256.f;    // a row's largest value
 
-// x * kHeld = hi + lo.
-__device__ __forceinline__ void split_held(float x, _Float16 &hi, _Float16 &lo)
-{
-    hi = (_Float16)(x * kHeld);
-    lo = (_Float16)fmaf(x, kHeld, -(float)hi);
-}
-
 // The largest magnitude of four values; NaN if one is.
 __device__ __forceinline__ float most(const f4 x)
 {
@@ -56,21 +49,30 @@ __device__ __forceinline__ float most(const f4 x)
                                          __builtin_elementwise_maximum(fabsf(x.z), fabsf(x.w)));
 }
 
-// Whether a row of LPR lanes, in any of the wave's 64 / LPR, has a largest value
-// that is not 0 and below kRowLow.
+// Rows lie in LPR lanes.  0 where one of the wave's 64 / LPR rows has no lane with
+// its bit in the mask.
+template <int LPR>
+__device__ __forceinline__ uint32_t every_row(unsigned long long mask)
+{
+    uint32_t lo = (uint32_t)mask, hi = (uint32_t)(mask >> 32);
+    if constexpr (LPR < 32) {
+        constexpr uint32_t one = LPR == 16 ? 0xFFFFu : 0xFFu;
+        uint32_t all = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = 0; i < 32; i += LPR) all = min(all, min(lo >> i & one, hi >> i & one));
+        return all;
+    }
+    return min(lo, hi);
+}
+
+// Whether a row, in any of the wave's, has a largest value that is not 0 and below kRowLow.
 template <int LPR>
 __device__ __forceinline__ bool low_row(float m)
 {
-    const unsigned long long ge = __ballot(m >= kRowLow);
+    const unsigned long long ge = __ballot(m >= kRowLow), pos = __ballot(m > 0.f);
     constexpr unsigned long long one = LPR == 32 ? 0xFFFFFFFFull : LPR == 16 ? 0xFFFFull : 0xFFull;
-    bool all = true;
-#pragma unroll
-    for (int i = 0; i < 64 / LPR; i++) all &= (ge >> (LPR * i) & one) != 0;
-    if (all) return false;
-    const unsigned long long pos = __ballot(m > 0.f);
     bool low = false;
-#pragma unroll
-    for (int i = 0; i < 64 / LPR; i++) low |= (pos >> (LPR * i) & one) != 0 && (ge >> (LPR * i) & one) == 0;
+    for (int i = 0; i < 64; i += LPR) low |= (pos >> i & one) != 0 && (ge >> i & one) == 0;
     return low;
 }
 
@@ -170,54 +172,44 @@ __global__ __launch_bounds__(256, 2) void attn_packed_k(PackedAttn a)
         }
     };
     auto store = [&](int b, int f) {
-        bool odd = false;
-        float big = 0.f;
+        float big = 0.f, m[4];
+        uint32_t rows = 0xFFFFFFFFu;
+        const int nl = stages_v ? 4 : KH;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (i >= nl) continue;
+            m[i] = most(ld[i]);
+            big = __builtin_elementwise_maximum(big, m[i]);
+            rows = min(rows, every_row<LPR>(__ballot(m[i] >= kRowLow)));
+        }
         if (stages_v) {
-            h4 hi[4], lo[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float m = most(ld[i]);
-                big = __builtin_elementwise_maximum(big, m);
-                odd |= low_row<LPR>(m);
-#pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    _Float16 h, l;
-                    split_held(ld[i][d], h, l);
-                    hi[d][i] = h;
-                    lo[d][i] = l;
-                }
-            }
-            if (mine) {
-                const int vb_ = x4 >> 3, at = 4 * (x4 & 7), sw = (x4 >> 2 & 1) + 2 * (vb_ & 1);
-#pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    ((h4 *)&S.v[b][0][vb_][vg][at + (d ^ sw)])[f] = hi[d];
-                    ((h4 *)&S.v[b][1][vb_][vg][at + (d ^ sw)])[f] = lo[d];
+            for (int d = 0; d < 4; d++) {
+                h2 hi[2], lo[2];
+                split2(ld[0][d], ld[1][d], kHeld, hi[0], lo[0]);
+                split2(ld[2][d], ld[3][d], kHeld, hi[1], lo[1]);
+                if (mine) {
+                    const int vb_ = x4 >> 3, at = 4 * (x4 & 7) + (d ^ ((x4 >> 2 & 1) + 2 * (vb_ & 1)));
+                    ((h4 *)&S.v[b][0][vb_][vg][at])[f] = h4{hi[0].x, hi[0].y, hi[1].x, hi[1].y};
+                    ((h4 *)&S.v[b][1][vb_][vg][at])[f] = h4{lo[0].x, lo[0].y, lo[1].x, lo[1].y};
                 }
             }
         } else {
 #pragma unroll
             for (int i = 0; i < KH; i++) {
-                const int r = kr + KS * (KH * f + i);
-                const float m = most(ld[i]);
-                big = __builtin_elementwise_maximum(big, m);
-                odd |= low_row<LPR>(m);
-                h4 hi, lo;
-#pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    _Float16 h, l;
-                    split_held(ld[i][d], h, l);
-                    hi[d] = h;
-                    lo[d] = l;
-                }
+                const int r = kr + KS * (KH * f + i), d8 = x4 >> 1;
+                h2 hi[2], lo[2];
+                split2(ld[i][0], ld[i][1], kHeld, hi[0], lo[0]);
+                split2(ld[i][2], ld[i][3], kHeld, hi[1], lo[1]);
                 if (mine && (2 * KH * KS == 32 || r < 32)) {
-                    const int d8 = x4 >> 1;
-                    ((h4 *)&S.k[b][0][d8][r ^ (d8 & 15)])[x4 & 1] = hi;
-                    ((h4 *)&S.k[b][1][d8][r ^ (d8 & 15)])[x4 & 1] = lo;
+                    ((h4 *)&S.k[b][0][d8][r ^ (d8 & 15)])[x4 & 1] = h4{hi[0].x, hi[0].y, hi[1].x, hi[1].y};
+                    ((h4 *)&S.k[b][1][d8][r ^ (d8 & 15)])[x4 & 1] = h4{lo[0].x, lo[0].y, lo[1].x, lo[1].y};
                 }
             }
         }
-        odd |= __any(!(big < kRowHigh));
+        bool odd = __any(!(big < kRowHigh));
+        if (rows == 0)  // a row of small values, or of zeros
+            for (int i = 0; i < nl; i++) odd |= low_row<LPR>(i == 0 ? m[0] : i == 1 ? m[1] : i == 2 ? m[2] : m[3]);
         if (lane == 0) S.odd[b][f][wave] = odd;
     };
     load(0, 0);

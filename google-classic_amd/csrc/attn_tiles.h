@@ -28,18 +28,37 @@ constexpr float score_scale(int hd)
 // maximum's last place, the sum of the two could round to 16.)
 constexpr float kPShift = 7.5f, kMaxSlack = 7.f;
 
-// x = hi + lo, two values at a time (x - hi is exact in fp32).
+// The f16 halves of two values, x = hi + lo within 2^-22 |x|: a packed conversion
+// and two mixed fused multiply-adds (x - hi is exact in fp32), which the compiler
+// otherwise takes apart into conversions and subtractions.
+__device__ __forceinline__ void split2(float x, float y, h2 &hi, h2 &lo)
+{
+    hi = __builtin_convertvector((f2){x, y}, h2);
+    uint32_t l;
+    asm("v_fma_mixlo_f16 %0, %1, 1.0, -%2 op_sel_hi:[0,0,1]" : "=v"(l) : "v"(x), "v"(hi));
+    asm("v_fma_mixhi_f16 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(y), "v"(hi));
+    lo = __builtin_bit_cast(h2, l);
+}
+
+// The same of x times s (a power of two).
+__device__ __forceinline__ void split2(float x, float y, float s, h2 &hi, h2 &lo)
+{
+    uint32_t h, l;
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(h) : "v"(x), "s"(s));
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(h) : "v"(y), "s"(s));
+    asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(l) : "v"(x), "s"(s), "v"(h));
+    asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(y), "s"(s), "v"(h));
+    hi = __builtin_bit_cast(h2, h);
+    lo = __builtin_bit_cast(h2, l);
+}
+
 __device__ __forceinline__ void split8(const float x[8], h8 &hi, h8 &lo)
 {
+    h2 h[4], l[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const h2 h = __builtin_convertvector((f2){x[2 * i], x[2 * i + 1]}, h2);
-        const h2 l = __builtin_convertvector((f2){x[2 * i] - (float)h.x, x[2 * i + 1] - (float)h.y}, h2);
-        hi[2 * i] = h.x;
-        hi[2 * i + 1] = h.y;
-        lo[2 * i] = l.x;
-        lo[2 * i + 1] = l.y;
-    }
+    for (int i = 0; i < 4; i++) split2(x[2 * i], x[2 * i + 1], h[i], l[i]);
+    hi = h8{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
+    lo = h8{l[0].x, l[0].y, l[1].x, l[1].y, l[2].x, l[2].y, l[3].x, l[3].y};
 }
 
 }  // namespace holo
