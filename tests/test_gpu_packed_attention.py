@@ -66,6 +66,30 @@ def test_packed_attention(holo, hd, heads, n_kv, rows, lds):
     assert np.array_equal(got, run(holo, q, k, v, rows, hd, heads, n_kv, lds))
 
 
+@pytest.mark.parametrize("hd,heads,n_kv,rows", [
+    (128, 64, 64, [1030]), (96, 32, 16, [1025, 300, 1000]), (128, 16, 4, [600, 33]), (96, 4, 4, [1500]),
+    (32, 32, 32, [200] * 9), (128, 8, 8, [65] * 50),
+], ids=str)
+def test_larger_batches(holo, hd, heads, n_kv, rows):
+    """Long prompts and many columns, on some of the rows and heads."""
+    print(f"case packed larger hd {hd} heads {heads}/{n_kv} rows {rows[:3]}", flush=True)
+    rng = np.random.default_rng(1)
+    total = sum(rows)
+    q, k, v = inputs(sum(rows), total, hd, heads, n_kv)
+    got, at = run(holo, q, k, v, rows, hd, heads, n_kv), 0
+    assert np.isfinite(got).all()
+    for n in rows[:3]:
+        for h in {0, heads - 1, int(rng.integers(heads))}:
+            g = h * n_kv // heads
+            kh, vh = (x[at:at + n, g * hd:(g + 1) * hd].astype(np.float64) for x in (k, v))
+            s = q[at:at + n, h * hd:(h + 1) * hd].astype(np.float64) @ kh.T / np.sqrt(hd)
+            s[np.arange(n)[None] > np.arange(n)[:, None]] = -np.inf
+            p = np.exp(s - s.max(1, keepdims=True))
+            want = (p / p.sum(1, keepdims=True)) @ vh
+            assert normwise(got[at:at + n, h * hd:(h + 1) * hd], want) <= TOL
+        at += n
+
+
 def test_agrees_with_one_sequence_at_a_time(holo):
     """holo_attention_prefill of each sequence from position 0."""
     print("case packed against prefill", flush=True)
