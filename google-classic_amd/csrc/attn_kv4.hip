@@ -29,55 +29,63 @@
 
 namespace holo {
 
-// The 8 values of a word as an MFMA operand; d and d24 = -24 d of the pairs (2 p, 2 p + 1).
-__device__ __forceinline__ h8 kv4_unpack(uint32_t w, const h2 d[4], const h2 d24[4])
+// The 8 values of a word as an MFMA operand; d and d24 = -24 d of the pairs (2 p,
+// 2 p + 1).  k16: 0x4C004C00, f16's 16 twice, in a register (v_and_or_b32 takes
+// one constant).
+__device__ __forceinline__ h8 kv4_unpack(uint32_t w, uint32_t k16, const h2 d[4], const h2 d24[4])
 {
     h2 x[4];
 #pragma unroll
     for (int p = 0; p < 4; p++) {
         const uint32_t n = p < 2 ? w << (6 - 4 * p) : w >> (4 * p - 6);
-        x[p] = __builtin_elementwise_fma(__builtin_bit_cast(h2, (n & 0x03C003C0u) | 0x4C004C00u), d[p], d24[p]);
+        x[p] = __builtin_elementwise_fma(__builtin_bit_cast(h2, (n & 0x03C003C0u) | k16), d[p], d24[p]);
     }
     return h8{x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
 }
 
-// A tile in a lane's registers.
+// A tile's keys and values in a lane's registers.
 template <int NB>
-struct Tile {
-    uint32_t k[2][NB], v[2 * NB];
-    uint16_t ks[2][NB];  // the scale of each K word's block
-    u4 vs[NB];
+struct TileK {
+    uint32_t w[2][NB], s[NB];  // s: the scales of word j of both halves' positions
+};
+template <int NB>
+struct TileV {
+    uint32_t w[2 * NB];
+    u4 s[NB];
 };
 
 template <int NB>
-__device__ __forceinline__ void load_tile(Tile<NB> &t, const uint8_t *at, int lane)
+__device__ __forceinline__ void load_k(TileK<NB> &t, const uint8_t *at, uint32_t lane)
 {
-    constexpr int HD = 32 * NB, W = NB % 2 ? 2 : 4;
-    const int r = lane & 15, g = lane >> 4;
+    const uint32_t r = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const uint32_t *k = (const uint32_t *)at + (64 * h + lane) * NB;
-        if constexpr (NB == 4) *(u4 *)t.k[h] = *(const u4 *)k;
-        else if constexpr (NB == 2) *(uint2 *)t.k[h] = *(const uint2 *)k;
+        const uint32_t *k = (const uint32_t *)(at + 4 * NB * (64 * h + lane));
+        if constexpr (NB == 4) *(u4 *)t.w[h] = *(const u4 *)k;
+        else if constexpr (NB == 2) *(uint2 *)t.w[h] = *(const uint2 *)k;
         else
 #pragma unroll
-            for (int j = 0; j < NB; j++) t.k[h][j] = k[j];
+            for (int j = 0; j < NB; j++) t.w[h][j] = k[j];
     }
-    const uint32_t *v = (const uint32_t *)(at + 16 * HD);
-#pragma unroll
-    for (int c = 0; c < 2 * NB / W; c++) {
-        if constexpr (W == 4) *(u4 *)(t.v + 4 * c) = *(const u4 *)(v + (64 * c + lane) * 4);
-        else *(uint2 *)(t.v + 2 * c) = *(const uint2 *)(v + (64 * c + lane) * 2);
-    }
-    const uint32_t *ks = (const uint32_t *)(at + 32 * HD);
 #pragma unroll
     for (int j = 0; j < NB; j++) {
-        const uint32_t s = ks[16 * ((NB * g + j) >> 2) + r];
-        t.ks[0][j] = (uint16_t)s;
-        t.ks[1][j] = (uint16_t)(s >> 16);
+        if (j > 0 && NB % 4 == 0) t.s[j] = t.s[0];  // one block a lane
+        else t.s[j] = *(const uint32_t *)(at + 1024 * NB + 4 * (16 * ((NB * g + j) >> 2) + r));
+    }
+}
+
+template <int NB>
+__device__ __forceinline__ void load_v(TileV<NB> &t, const uint8_t *at, uint32_t lane)
+{
+    constexpr int W = NB % 2 ? 2 : 4;
+#pragma unroll
+    for (int c = 0; c < 2 * NB / W; c++) {
+        const uint8_t *v = at + 512 * NB + 4 * W * (64 * c + lane);
+        if constexpr (W == 4) *(u4 *)(t.w + 4 * c) = *(const u4 *)v;
+        else *(uint2 *)(t.w + 2 * c) = *(const uint2 *)v;
     }
 #pragma unroll
-    for (int b = 0; b < NB; b++) t.vs[b] = *(const u4 *)(at + 34 * HD + 64 * b + 16 * g);
+    for (int b = 0; b < NB; b++) t.s[b] = *(const u4 *)(at + 1088 * NB + 64 * b + 16 * (lane >> 4));
 }
 
 struct Kv4Attn {
@@ -94,7 +102,7 @@ struct Kv4Attn {
 // Column c of an entry and KV head: row c / G, query head kvh * G + c % G.
 // Waves: W; the columns of a workgroup: 16.
 template <int NB, int W>
-__global__ __launch_bounds__(64 * W) void attn_kv4_k(Kv4Attn a)
+__global__ __launch_bounds__(64 * W, 2) void attn_kv4_k(Kv4Attn a)
 {
     constexpr int HD = 32 * NB, OS = HD + 4;
     __shared__ __align__(16) float lo_[W][16][OS];
@@ -114,10 +122,9 @@ __global__ __launch_bounds__(64 * W) void attn_kv4_k(Kv4Attn a)
     if (t0 >= ntiles && blockIdx.x > 0) return;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int col = c0 + r;
-    const bool valid = col < ncols;
-    const int row = valid ? col / G : 0, head = kvh * G + (valid ? col % G : 0);
-    const int qpos = valid ? from + row : -1;  // the column sees positions 0 .. qpos
+    const int col = min(c0 + r, ncols - 1);  // past the last: the last again
+    const int row = col / G, head = kvh * G + col % G;
+    const int qpos = from + row;               // the column sees positions 0 .. qpos
     const int all = from + first_row;          // positions 0 .. all are seen by every column
 
     // q of the column: dims 8 (NB g + j) .. + 7 in step j, scaled to [2^13, 2^14)
@@ -128,8 +135,7 @@ __global__ __launch_bounds__(64 * W) void attn_kv4_k(Kv4Attn a)
         const float *qp = a.q + (int64_t)(e.first + row) * a.ldq + (int64_t)head * HD + 8 * NB * g;
 #pragma unroll
         for (int j = 0; j < NB; j++) {
-            const float4 u = valid ? *(const float4 *)(qp + 8 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float4 w = valid ? *(const float4 *)(qp + 8 * j + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 u = *(const float4 *)(qp + 8 * j), w = *(const float4 *)(qp + 8 * j + 4);
             x[j][0] = u.x, x[j][1] = u.y, x[j][2] = u.z, x[j][3] = u.w;
             x[j][4] = w.x, x[j][5] = w.y, x[j][6] = w.z, x[j][7] = w.w;
 #pragma unroll
@@ -152,60 +158,119 @@ __global__ __launch_bounds__(64 * W) void attn_kv4_k(Kv4Attn a)
     }
 
     float m = -FLT_MAX, l = 0.f;  // of log2 units; l: this lane's positions
-    f4 o[2 * NB];
+    f4 o[2 * NB], s[2];
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) o[i] = f4{};
-
-    for (int t = t0 + wave; t < t1; t += W) {
-        const uint8_t *at = kv4_tile<NB>(a.c, e, kvh, t);
-        if (!at) continue;  // no page: positions that nobody sees
-        Tile<NB> x;
-        load_tile<NB>(x, at, lane);
-        f4 s[2] = {f4{}, f4{}};
+    uint32_t k16;
+    asm("v_mov_b32 %0, 0x4C004C00" : "=v"(k16));
+    // Tile t (past the range: its last); there: whether it has a page, else the
+    // pool's first tile stands for it and nobody sees it.
+    auto where = [&](int t, bool &there) {
+        const uint8_t *at = kv4_tile<NB>(a.c, e, kvh, min(t, t1 - 1));
+        there = at != nullptr;
+        return there ? at : a.c.pool;
+    };
+    TileK<NB> xk;
+    TileV<NB> xv;
+    auto scores = [&]() {
+        s[0] = s[1] = f4{};
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int j = 0; j < NB; j++) {
+            const h2 both = __builtin_bit_cast(h2, xk.s[j]);
 #pragma unroll
-            for (int j = 0; j < NB; j++) {
-                const _Float16 d = __builtin_bit_cast(_Float16, x.ks[h][j]);
-                const h2 dd = {d, d}, dm = dd * (_Float16)-24.f;
+            for (int h = 0; h < 2; h++) {
+                const h2 dd = {both[h], both[h]}, dm = dd * (_Float16)-24.f;
                 const h2 d4[4] = {dd, dd, dd, dd}, m4[4] = {dm, dm, dm, dm};
-                const h8 k8 = kv4_unpack(x.k[h][j], d4, m4);
+                const h8 k8 = kv4_unpack(xk.w[h][j], k16, d4, m4);
                 s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[j], s[h], 0, 0, 0);
                 s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[j], s[h], 0, 0, 0);
             }
-        float p[8];
+        }
+    };
+    // Some column does not see the whole tile.  Its probability is 0 where it does
+    // not; the values there must be finite then: a scale past the end, or a NaN that
+    // some column does not see, becomes 0, and a column that sees the NaN takes it here.
+    auto mask = [&](int t, bool there) {
+        const int sees = there ? qpos : -1, all_see = there ? all : -1;
 #pragma unroll
-        for (int i = 0; i < 8; i++) p[i] = s[i >> 2][i & 3] * sc;
-        const int p0 = 32 * t;
-        if (p0 + 31 > all) {
-            // some column does not see the whole tile.  Its probability is 0 where it
-            // does not; the values there must be finite then: a scale past the end, or a NaN
-            // that some column does not see, becomes 0, and a column that sees the NaN
-            // takes it here.
+        for (int i = 0; i < 8; i++)
+            if (32 * t + v_pos(g, i) > sees) s[i >> 2][i & 3] = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            h8 d = __builtin_bit_cast(h8, xv.s[b]);
+            int nan = 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const int pos = p0 + v_pos(g, i);
-                if (pos > qpos) p[i] = -INFINITY;
+                const int pos = 32 * t + v_pos(g, i);
+                const bool is = d[i] != d[i];
+                nan |= is && pos <= sees;
+                if (!there || pos >= e.len || (is && pos > all_see)) d[i] = (_Float16)0.f;
             }
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                h8 d = __builtin_bit_cast(h8, x.vs[b]);
-                int nan = 0;
+            xv.s[b] = __builtin_bit_cast(u4, d);
+            nan |= __shfl_xor(nan, 16, 64);
+            nan |= __shfl_xor(nan, 32, 64);
+            if (nan) o[2 * b] = o[2 * b + 1] = f4{NAN, NAN, NAN, NAN};
+        }
+    };
+    auto most = [&]() {
+        return sc * fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    };
+    int t = t0 + wave;
+    if (t < t1) {
+        // Two tiles under way: keys are loaded a tile ahead of the values, each into
+        // the registers that the products have just read.
+        bool there, there1;
+        const uint8_t *at = where(t, there), *at1 = where(t + W, there1);
+        load_k<NB>(xk, at, lane);
+        load_v<NB>(xv, at, lane);
+        scores();
+        load_k<NB>(xk, at1, lane);
+        bool masked = false;  // this tile's scores are
+        // Tiles that leave the maximum alone, in a loop of their own: with the scaling
+        // of the outputs in it the compiler copied them every tile.
+        for (;;) {
+            for (; t < t1; t += W) {
+                if ((32 * t + 31 > all || !there) && !masked) {
+                    mask(t, there);
+                    masked = true;
+                }
+                if (__any(most() > m + kMaxSlack)) break;
+                bool there2;
+                const uint8_t *at2 = where(t + 2 * W, there2);
+                float p[8], ps[2] = {};
+                const float off = kPShift - m;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const int pos = p0 + v_pos(g, i);
-                    const bool is = d[i] != d[i];
-                    nan |= is && pos <= qpos;
-                    if (pos >= e.len || (is && pos > all)) d[i] = (_Float16)0.f;
+                    p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], sc, off));
+                    ps[i & 1] += p[i];
                 }
-                x.vs[b] = __builtin_bit_cast(u4, d);
-                nan |= __shfl_xor(nan, 16, 64);
-                nan |= __shfl_xor(nan, 32, 64);
-                if (nan) o[2 * b] = o[2 * b + 1] = f4{NAN, NAN, NAN, NAN};
+                l += ps[0] + ps[1];
+                h8 ph, pl;
+                split8(p, ph, pl);
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    h2 d4[4], m4[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        d4[i] = __builtin_bit_cast(h2, (uint32_t)xv.s[b][i]);
+                        m4[i] = d4[i] * (_Float16)-24.f;
+                    }
+#pragma unroll
+                    for (int i = 2 * b; i < 2 * b + 2; i++) {
+                        const h8 v8 = kv4_unpack(xv.w[i], k16, d4, m4);
+                        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[i], 0, 0, 0);
+                        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[i], 0, 0, 0);
+                    }
+                }
+                load_v<NB>(xv, at1, lane);
+                scores();
+                load_k<NB>(xk, at2, lane);
+                there = there1, there1 = there2, at1 = at2;
+                masked = false;
             }
-        }
-        float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-        if (__any(mx > m + kMaxSlack)) {
+            if (t >= t1) break;
+            float mx = most();
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
             const float w = __builtin_amdgcn_exp2f(m - mx);
@@ -213,30 +278,6 @@ __global__ __launch_bounds__(64 * W) void attn_kv4_k(Kv4Attn a)
             l *= w;
 #pragma unroll
             for (int i = 0; i < 2 * NB; i++) o[i] *= w;
-        }
-        float ps = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            p[i] = __builtin_amdgcn_exp2f(p[i] - m + kPShift);
-            ps += p[i];
-        }
-        l += ps;
-        h8 ph, pl;
-        split8(p, ph, pl);
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            h2 d4[4], m4[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                d4[i] = __builtin_bit_cast(h2, (uint32_t)x.vs[b][i]);
-                m4[i] = d4[i] * (_Float16)-24.f;
-            }
-#pragma unroll
-            for (int i = 2 * b; i < 2 * b + 2; i++) {
-                const h8 v8 = kv4_unpack(x.v[i], d4, m4);
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[i], 0, 0, 0);
-            }
         }
     }
 
@@ -282,11 +323,14 @@ __global__ __launch_bounds__(64 * W) void attn_kv4_k(Kv4Attn a)
     }
 }
 
-// Joins the ranges of a row and head, in range order.
+// Joins the ranges of a row and head, in range order: groups of HD / 4 lanes take
+// every 256 / (HD / 4)-th range, four dims a lane, and meet in LDS in group order.
 template <int NB>
-__global__ __launch_bounds__(64) void attn_kv4_join_k(Kv4Attn a)
+__global__ __launch_bounds__(256) void attn_kv4_join_k(Kv4Attn a)
 {
-    constexpr int HD = 32 * NB, D = HD / 4;  // a lane's four dims
+    constexpr int HD = 32 * NB, D = HD / 4, GR = 256 / D, R = 4;
+    __shared__ __align__(16) float lo_[GR][HD];
+    __shared__ float lm[GR], ll[GR];
     const Kv4Entry e = kv4_entry(a.c, a.b, blockIdx.z);
     const int h = blockIdx.x, row = blockIdx.y;
     if (row >= e.take || e.len > a.b.max_len) return;
@@ -298,17 +342,52 @@ __global__ __launch_bounds__(64) void attn_kv4_join_k(Kv4Attn a)
     if (n <= 1) return;
     const int64_t at = e.first + row;
     const float *pp = a.part + ((at * a.n_heads + h) * a.splits) * (HD + 4);
-    float M = -FLT_MAX;
-    for (int s = 0; s < n; s++) M = fmaxf(M, pp[s * (HD + 4) + HD]);
-    if (threadIdx.x >= D) return;
-    float L = 0.f;
+    const int g = threadIdx.x / D, d = 4 * (threadIdx.x % D);
+    float M = -FLT_MAX, L = 0.f;
     f4 O = f4{};
-    for (int s = 0; s < n; s++) {
-        const float f = __builtin_amdgcn_exp2f(pp[s * (HD + 4) + HD] - M);
-        L = fmaf(f, pp[s * (HD + 4) + HD + 1], L);
-        O += f * *(const f4 *)(pp + s * (HD + 4) + 4 * threadIdx.x);
+    if (g < GR) {
+        for (int s0 = g; s0 < n; s0 += R * GR) {
+            f2 ml[R];
+            f4 x[R];
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const float *p = pp + (int64_t)min(s0 + GR * i, n - 1) * (HD + 4);
+                ml[i] = *(const f2 *)(p + HD);
+                x[i] = *(const f4 *)(p + d);
+            }
+            float mx = M;
+#pragma unroll
+            for (int i = 0; i < R; i++) mx = fmaxf(mx, ml[i].x);  // the last range twice does no harm here
+            const float was = __builtin_amdgcn_exp2f(M - mx);
+            M = mx;
+            L *= was;
+            O *= was;
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                if (s0 + GR * i >= n) continue;
+                const float f = __builtin_amdgcn_exp2f(ml[i].x - M);
+                L = fmaf(f, ml[i].y, L);
+                O += f * x[i];
+            }
+        }
+        *(f4 *)&lo_[g][d] = O;
+        if (d == 0) {
+            lm[g] = M;
+            ll[g] = L;
+        }
     }
-    *(f4 *)(a.out + at * a.ldo + (int64_t)h * HD + 4 * threadIdx.x) = O * (L == 0.f ? 0.f : 1.0f / L);
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    const int groups = min(n, GR);
+    for (int i = 0; i < groups; i++) M = fmaxf(M, lm[i]);
+    L = 0.f;
+    O = f4{};
+    for (int i = 0; i < groups; i++) {
+        const float f = __builtin_amdgcn_exp2f(lm[i] - M);
+        L = fmaf(f, ll[i], L);
+        O += f * *(const f4 *)&lo_[i][d];
+    }
+    *(f4 *)(a.out + at * a.ldo + (int64_t)h * HD + d) = O * (L == 0.f ? 0.f : 1.0f / L);
 }
 
 // Tiles of a range: all of a sequence where the launch has two workgroups a CU
@@ -344,7 +423,7 @@ static int run_attn(Kv4Attn a)
     }
     hipLaunchKernelGGL((attn_kv4_k<NB, W>), grid, dim3(64 * W), 0, stream(), a);
     HOLO_LAUNCH_CHECK();
-    hipLaunchKernelGGL(attn_kv4_join_k<NB>, dim3(a.n_heads, take, a.b.n_seqs), dim3(64), 0, stream(), a);
+    hipLaunchKernelGGL(attn_kv4_join_k<NB>, dim3(a.n_heads, take, a.b.n_seqs), dim3(256), 0, stream(), a);
     HOLO_LAUNCH_CHECK();
     return 0;
 }
