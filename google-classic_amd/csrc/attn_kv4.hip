@@ -102,11 +102,12 @@ struct Kv4Attn {
 // Column c of an entry and KV head: row c / G, query head kvh * G + c % G.
 // Waves: W; the columns of a workgroup: 16.
 template <int NB, int W>
-__global__ __launch_bounds__(64 * W, 2) void attn_kv4_k(Kv4Attn a)
+__global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
 {
     constexpr int HD = 32 * NB, OS = HD + 4;
-    __shared__ __align__(16) float lo_[W][16][OS];
-    __shared__ float lm[W][16], ll[W][16];
+    extern __shared__ __align__(16) float kv4_lds[];
+    float(*lo_)[16][OS] = (float(*)[16][OS])kv4_lds;
+    float(*lm)[16] = (float(*)[16])(kv4_lds + W * 16 * OS), (*ll)[16] = lm + W;
     const int kvh = blockIdx.y / a.ctiles, ct = blockIdx.y % a.ctiles;
     const int G = a.n_heads / a.c.n_kv_heads;
     const Kv4Entry e = kv4_entry(a.c, a.b, blockIdx.z);
@@ -188,28 +189,45 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_k(Kv4Attn a)
         }
     };
     // Some column does not see the whole tile.  Its probability is 0 where it does
-    // not; the values there must be finite then: a scale past the end, or a NaN that
-    // some column does not see, becomes 0, and a column that sees the NaN takes it here.
+    // not; the values there must be finite then: scales past the sequence's end (and
+    // of a tile without a page) become 0, and a NaN's that some column does not see,
+    // the columns that see it taking the NaN at the end.  (Twice changes nothing.)
+    int poison = 0;  // by block of dims: this lane's positions have a NaN that the column sees
     auto mask = [&](int t, bool there) {
-        const int sees = there ? qpos : -1, all_see = there ? all : -1;
+        const int sees = (there ? qpos : -1) - 32 * t, end = there ? e.len - 32 * t : 0;
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (32 * t + v_pos(g, i) > sees) s[i >> 2][i & 3] = -INFINITY;
+            if (v_pos(g, i) > sees) s[i >> 2][i & 3] = -INFINITY;
+        uint32_t keep[4];  // of the lane's positions, two a register
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            h8 d = __builtin_bit_cast(h8, xv.s[b]);
-            int nan = 0;
+        for (int i = 0; i < 4; i++) {
+            const int left = end - v_pos(g, 2 * i);
+            keep[i] = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u;
+        }
+        h2 sum = {};
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int pos = 32 * t + v_pos(g, i);
-                const bool is = d[i] != d[i];
-                nan |= is && pos <= sees;
-                if (!there || pos >= e.len || (is && pos > all_see)) d[i] = (_Float16)0.f;
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                xv.s[b][i] &= keep[i];
+                sum += __builtin_bit_cast(h2, (uint32_t)xv.s[b][i]);
             }
-            xv.s[b] = __builtin_bit_cast(u4, d);
-            nan |= __shfl_xor(nan, 16, 64);
-            nan |= __shfl_xor(nan, 32, 64);
-            if (nan) o[2 * b] = o[2 * b + 1] = f4{NAN, NAN, NAN, NAN};
+        const _Float16 all_of = sum.x + sum.y;
+        if (__builtin_expect(__any(all_of != all_of), 0)) {
+            const int all_see = all - 32 * t;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                h8 d = __builtin_bit_cast(h8, xv.s[b]);
+                int nan = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const bool is = d[i] != d[i];
+                    nan |= is && v_pos(g, i) <= sees;
+                    if (is && v_pos(g, i) > all_see) d[i] = (_Float16)0.f;
+                }
+                xv.s[b] = __builtin_bit_cast(u4, d);
+                poison |= nan << b;
+            }
         }
     };
     auto most = [&]() {
@@ -226,15 +244,11 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_k(Kv4Attn a)
         load_v<NB>(xv, at, lane);
         scores();
         load_k<NB>(xk, at1, lane);
-        bool masked = false;  // this tile's scores are
         // Tiles that leave the maximum alone, in a loop of their own: with the scaling
         // of the outputs in it the compiler copied them every tile.
         for (;;) {
             for (; t < t1; t += W) {
-                if ((32 * t + 31 > all || !there) && !masked) {
-                    mask(t, there);
-                    masked = true;
-                }
+                if (32 * t + 31 > all || !there) mask(t, there);
                 if (__any(most() > m + kMaxSlack)) break;
                 bool there2;
                 const uint8_t *at2 = where(t + 2 * W, there2);
@@ -267,7 +281,6 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_k(Kv4Attn a)
                 scores();
                 load_k<NB>(xk, at2, lane);
                 there = there1, there1 = there2, at1 = at2;
-                masked = false;
             }
             if (t >= t1) break;
             float mx = most();
@@ -284,6 +297,13 @@ __global__ __launch_bounds__(64 * W, 2) void attn_kv4_k(Kv4Attn a)
     // the waves meet: O = sum_w 2^(m_w - M) O_w
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
+    if (__any(poison)) {
+        poison |= __shfl_xor(poison, 16, 64);
+        poison |= __shfl_xor(poison, 32, 64);
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++)
+            if (poison >> (i >> 1) & 1) o[i] = f4{NAN, NAN, NAN, NAN};
+    }
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) *(f4 *)&lo_[wave][r][16 * i + 4 * g] = o[i];
     if (g == 0) {
@@ -390,19 +410,24 @@ __global__ __launch_bounds__(256) void attn_kv4_join_k(Kv4Attn a)
     *(f4 *)(a.out + at * a.ldo + (int64_t)h * HD + d) = O * (L == 0.f ? 0.f : 1.0f / L);
 }
 
-// Tiles of a range: all of a sequence where the launch has two workgroups a CU
-// without ranges, else as many ranges as bring it there, of at least 4 tiles.
+// Tiles of a range: all of a sequence where it has few (700 positions of 32
+// sequences, a workgroup a CU: 9.7 us, in two ranges 13.4, the launch that joins
+// them among it; 513 of one: 8.5, in three 8.9) or where there are two workgroups
+// a CU without ranges (64 sequences of up to 8192: 104, in ranges of 4096
+// positions 118); else as many ranges as bring it there, of at least 8 tiles (one
+// of 8000: 10.1, of at least 4 12.2).
 static int range_tiles(int64_t groups, int tiles)
 {
+    if (tiles <= 24) return 24;
     const int64_t want = (2 * (int64_t)num_cus() + groups - 1) / groups;
     const int64_t chunk = (tiles + want - 1) / want;
-    return (int)(chunk < 4 ? 4 : chunk);
+    return (int)(chunk < 8 ? 8 : chunk);
 }
 
 template <int NB>
 static int run_attn(Kv4Attn a)
 {
-    constexpr int W = 4;
+    constexpr int W = 4;  // (eight: 64 sequences 119 us, 513 positions of one 9.2)
     const int G = a.n_heads / a.c.n_kv_heads, take = a.b.max_rows;
     a.ctiles = (int)(((int64_t)take * G + 15) / 16);
     const int tiles = (a.b.max_len + 31) / 32;
@@ -410,8 +435,15 @@ static int run_attn(Kv4Attn a)
     a.chunk = range_tiles(groups, tiles);
     a.splits = max(1, (tiles + a.chunk - 1) / a.chunk);
     const dim3 grid(a.splits, a.ctiles * a.c.n_kv_heads, a.b.n_seqs);
+    constexpr size_t lds = (size_t)W * 16 * (32 * NB + 4 + 2) * sizeof(float);
+    static bool attr = false;
+    if (!attr) {
+        HOLO_CHECK(hipFuncSetAttribute((const void *)attn_kv4_k<NB, W>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)lds));
+        attr = true;
+    }
     if (a.splits == 1) {
-        hipLaunchKernelGGL((attn_kv4_k<NB, W>), grid, dim3(64 * W), 0, stream(), a);
+        hipLaunchKernelGGL((attn_kv4_k<NB, W>), grid, dim3(64 * W), lds, stream(), a);
         HOLO_LAUNCH_CHECK();
         return 0;
     }
@@ -421,7 +453,7 @@ static int run_attn(Kv4Attn a)
         latch_error((int)hipErrorOutOfMemory, "holo_attention_kv4: partial sums", __FILE__, __LINE__);
         return (int)hipErrorOutOfMemory;
     }
-    hipLaunchKernelGGL((attn_kv4_k<NB, W>), grid, dim3(64 * W), 0, stream(), a);
+    hipLaunchKernelGGL((attn_kv4_k<NB, W>), grid, dim3(64 * W), lds, stream(), a);
     HOLO_LAUNCH_CHECK();
     hipLaunchKernelGGL(attn_kv4_join_k<NB>, dim3(a.n_heads, take, a.b.n_seqs), dim3(256), 0, stream(), a);
     HOLO_LAUNCH_CHECK();
