@@ -147,8 +147,7 @@ __global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
         }
         big = fmaxf(big, __shfl_xor(big, 16, 64));
         big = fmaxf(big, __shfl_xor(big, 32, 64));
-        // rows of zeros, and rows with an infinity (whose halves make NaN of it), as they are
-        const int ex = big > 0.f && big <= FLT_MAX ? ilogbf(big) - 13 : 0;
+        const int ex = scale_exp(big);
 #pragma unroll
         for (int j = 0; j < NB; j++) {
 #pragma unroll

@@ -38,9 +38,6 @@
 
 namespace holo {
 
-typedef float f16v __attribute__((ext_vector_type(16)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-
 struct PackedAttn {
     holo_batch_t b;
     float *out;
@@ -75,13 +72,6 @@ __device__ __forceinline__ bool some_low(const float (&m)[N])
         bits = r[0] | r[1];
     }
     return __any(bits != (1 << N) - 1);
-}
-
-// The larger of the two lanes j and j + 32.
-__device__ __forceinline__ float max_halves(float v)
-{
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // Whether a row, in any of the wave's, has a largest value that is not 0 and below kRowLow.
@@ -257,9 +247,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
                 big = fmaxf(big, fabsf(x[c][i]));
             }
         }
-        big = fmaxf(big, __shfl_xor(big, 32, 64));
-        // to [2^13, 2^14); rows of zeros, and rows with an infinity (whose halves make NaN of it), as they are
-        const int ex = big > 0.f && big <= FLT_MAX ? ilogbf(big) - 13 : 0;
+        const int ex = scale_exp(max_halves(big));
 #pragma unroll
         for (int c = 0; c < NC; c++) {
 #pragma unroll
@@ -568,7 +556,7 @@ __global__ __launch_bounds__(64 * W, 8 / W) void attn_packed_split_k(PackedAttn 
             float big = fmaxf(fmaxf(fabsf(x[i][0]), fabsf(x[i][1])), fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
 #pragma unroll
             for (int y = 1; y < QL; y <<= 1) big = fmaxf(big, __shfl_xor(big, y, 64));
-            const int ex = big > 0.f && big <= FLT_MAX ? ilogbf(big) - 13 : 0;
+            const int ex = scale_exp(big);
 #pragma unroll
             for (int y = 0; y < 4; y++) x[i][y] = ldexpf(x[i][y], -ex);
             h2 hi[2], lo[2];

@@ -1,5 +1,5 @@
-// attn_tiles.h -- what the attention kernels on 16-column tiles share: operand
-// types of v_mfma_f32_16x16x32_f16, the split of fp32 values into two f16 halves,
+// attn_tiles.h -- what the attention kernels on the matrix cores share: operand
+// types of v_mfma_f32_16x16x32_f16 and v_mfma_f32_32x32x16_f16, the split of fp32 values into two f16 halves,
 // and the softmax's scale.
 #pragma once
 
@@ -10,9 +10,11 @@
 namespace holo {
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 // Scores are in log2 units.  q is multiplied by this before it is split: what is
@@ -21,6 +23,14 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr float score_scale(int hd)
 {
     return hd == 32 ? 0.25503486f : hd == 64 ? 0.18033688f : hd == 96 ? 0.14724444f : 0.12751743f;  // log2(e) / sqrt(hd)
+}
+
+// The exponent by which a row of q is scaled down, its largest value to [2^13,
+// 2^14); rows of zeros, and rows with an infinity (whose halves make NaN of it), as
+// they are.  (-100: a power of two that multiplies scores is not 0.)
+__device__ __forceinline__ int scale_exp(float big)
+{
+    return big > 0.f && big <= FLT_MAX ? max(ilogbf(big) - 13, -100) : 0;
 }
 
 // Probabilities are held times 2^kPShift; a running maximum moves when a score
@@ -59,6 +69,13 @@ __device__ __forceinline__ void split8(const float x[8], h8 &hi, h8 &lo)
     for (int i = 0; i < 4; i++) split2(x[2 * i], x[2 * i + 1], h[i], l[i]);
     hi = h8{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
     lo = h8{l[0].x, l[0].y, l[1].x, l[1].y, l[2].x, l[2].y, l[3].x, l[3].y};
+}
+
+// The larger of the two lanes j and j + 32.
+__device__ __forceinline__ float max_halves(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 }  // namespace holo

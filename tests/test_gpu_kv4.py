@@ -172,6 +172,10 @@ def test_blocks_of_every_kind(holo):
     (32, 16, 1, 64, [90, 130], [33, 2]),
     (64, 40, 2, 32, [75], [7]),
     (128, 2, 2, 256, [300, 0, 290], [3, 2, 1]),
+    (64, 8, 1, 128, [1300, 900], [25, 40]),
+    (96, 6, 2, 64, [1000], [150]),
+    (32, 40, 40, 32, [200, 90], [70, 33]),
+    (128, 16, 2, 32, [140], [9]),
 ], ids=str)
 def test_attention_over_pages(holo, hd, heads, n_kv, page_len, lens, rows):
     print(f"case kv4 attention hd {hd} heads {heads}/{n_kv} page {page_len} lens {lens} rows {rows}", flush=True)
