@@ -17,49 +17,65 @@ namespace holo {
 // ---- quantisation of a block of 32 ----------------------------------------------------
 //
 // Eight lanes hold a block, four values each.  The code is the nearest integer
-// to x / d: rint(x * (1 / d)) is off by one at most where x lies next to the
-// middle of two codes, and the remainder x - c d (exact: c d has 12 bits and x
-// lies within a factor of c d) says which one it is.
+// to x / d.  x * (1 / d) is within 2^-20 of it, so its nearest integer is the code
+// unless it lies that near to the middle of two; there the remainder x - c d
+// decides (exact: c d has 12 bits and x lies within a factor of c d).
+
+// The larger (or smaller) of the eight lanes' values; NaN if one is.
+template <bool MAX>
+__device__ __forceinline__ float of_eight(float v)
+{
+    auto pick = [](float a, float b) { return MAX ? __builtin_elementwise_maximum(a, b) : __builtin_elementwise_minimum(a, b); };
+    v = pick(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false)));   // quad [1,0,3,2]
+    v = pick(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false)));   // quad [2,3,0,1]
+    return pick(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false)));  // half mirror
+}
 
 // f16 bits of the block's scale: bfloat16(|m| / 8), at most 2720, and m's sign
 // reversed; NaN where a value is not finite.
 __device__ __forceinline__ uint16_t kv4_scale(const float4 x)
 {
-    float lo = fminf(fminf(x.x, x.y), fminf(x.z, x.w)), hi = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
-    int bad = !(fabsf(x.x) <= FLT_MAX && fabsf(x.y) <= FLT_MAX && fabsf(x.z) <= FLT_MAX && fabsf(x.w) <= FLT_MAX);
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        lo = fminf(lo, __shfl_xor(lo, o, 64));
-        hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-        bad |= __shfl_xor(bad, o, 64);
-    }
-    if (bad) return 0x7E00;
-    const uint32_t u = __float_as_uint(fmaxf(-lo, hi) * 0.125f);
+    auto least = [](float a, float b) { return __builtin_elementwise_minimum(a, b); };
+    auto most = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };
+    const float lo = of_eight<false>(least(least(x.x, x.y), least(x.z, x.w)));
+    const float hi = of_eight<true>(most(most(x.x, x.y), most(x.z, x.w)));
+    const float big = most(-lo, hi);
+    const uint32_t u = __float_as_uint(big * 0.125f);
     const float b = __uint_as_float((u + 0x7FFFu + ((u >> 16) & 1u)) & 0xFFFF0000u);  // bfloat16, ties to even
     const float d = fminf(b, 2720.f);
-    return __builtin_bit_cast(uint16_t, (_Float16)(-lo >= hi ? d : -d));
-}
-
-__device__ __forceinline__ uint32_t kv4_code(float x, float d, float inv)
-{
-    float c = rintf(fminf(fmaxf(x * inv, -9.f), 9.f));
-    float r = fmaf(-c, d, x);
-    r = d < 0.f ? -r : r;
-    const float h = 0.5f * fabsf(d);
-    const bool odd = (int)c & 1;
-    if (r > h || (r == h && odd)) c += 1.f;
-    else if (r < -h || (r == -h && odd)) c -= 1.f;
-    return (uint32_t)((int)fminf(fmaxf(c, -8.f), 7.f) + 8);
+    const uint16_t h = __builtin_bit_cast(uint16_t, (_Float16)(-lo >= hi ? d : -d));
+    return big <= FLT_MAX ? h : (uint16_t)0x7E00;
 }
 
 // The lane's four codes, one a byte.
-__device__ __forceinline__ uint32_t kv4_codes(const float4 x, uint16_t scale)
+__device__ __forceinline__ uint32_t kv4_codes(const float4 x4, uint16_t scale)
 {
     const float d = (float)__builtin_bit_cast(_Float16, scale);
     if (!(fabsf(d) > 0.f)) return 0x08080808u;  // zeros, and blocks of NaN
-    const float inv = 1.0f / d;
-    return kv4_code(x.x, d, inv) | kv4_code(x.y, d, inv) << 8 | kv4_code(x.z, d, inv) << 16 |
-           kv4_code(x.w, d, inv) << 24;
+    const float inv = 1.0f / d, x[4] = {x4.x, x4.y, x4.z, x4.w};
+    float c[4];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float q = fminf(fmaxf(x[i] * inv, -9.f), 9.f);
+        c[i] = rintf(q);
+        near |= fabsf(q - c[i]) > 0.5f - 0x1p-16f;
+    }
+    if (near) {
+        const float h = 0.5f * fabsf(d);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float r = fmaf(-c[i], d, x[i]);
+            r = d < 0.f ? -r : r;
+            const bool odd = (int)c[i] & 1;
+            if (r > h || (r == h && odd)) c[i] += 1.f;
+            else if (r < -h || (r == -h && odd)) c[i] -= 1.f;
+        }
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w |= (uint32_t)((int)fminf(fmaxf(c[i], -8.f), 7.f) + 8) << (8 * i);
+    return w;
 }
 
 // Words of V in a tile, and the place of word (m, lane g, r) among them.
@@ -82,14 +98,20 @@ struct VWords {
 // A workgroup takes one tile of one KV head of an entry: groups of eight lanes
 // quantise (position, block) pairs, the keys straight into their words (a pair
 // of lanes makes one), the values through LDS, because a word of V holds eight
-// positions of a dim.  A word of V with positions outside the batch keeps their
-// nibbles.  Nothing but the tile is written, so no two workgroups meet.
+// positions of a dim.  There the codes lie as bytes, the dims r + 16 m of an r side
+// by side, so that a thread reads the VW dims of its words for each of the eight
+// positions and turns bytes into words by byte permutes.  A word of V with
+// positions outside the batch keeps their nibbles; it is loaded with the rows.
+// Nothing but the tile is written, so no two workgroups meet.
+//
+// What bounds it: for four prompts of up to 1000 rows the instructions of the
+// quantisation; for single rows the chain of loads (lengths, page, rows).
 template <int NB>
 __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, const float *k, const float *v, int ldk,
                                                     int ldv)
 {
-    constexpr int HD = 32 * NB;
-    __shared__ __align__(16) uint8_t lv[32][HD];
+    constexpr int HD = 32 * NB, VW = VWords<NB>::W, M = 2 * NB;
+    __shared__ __align__(16) uint8_t lv[32][HD];  // [position][16 r's][M dims r + 16 m]
     const Kv4Entry e = kv4_entry(c, b, blockIdx.z);
     const int kvh = blockIdx.y, from = e.len - e.rows;  // position of the entry's first row
     const int t = (max(from, 0) >> 5) + blockIdx.x, p0 = 32 * t;
@@ -100,6 +122,17 @@ __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, c
     if (!tile) return;
     uint32_t *kw = (uint32_t *)tile, *vw = (uint32_t *)(tile + 16 * HD);
     uint16_t *ks = (uint16_t *)(tile + 32 * HD), *vs = (uint16_t *)(tile + 34 * HD);
+    // the thread's words of V, VW of lane group vg, and which of their nibbles are new
+    const int vg = threadIdx.x >> 4 & 3, vr = threadIdx.x & 15, vc = threadIdx.x >> 6;
+    uint32_t mask = 0, old[VW] = {};
+    if (VW * vc < M) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (v_pos(vg, j) >= lo && v_pos(vg, j) < hi) mask |= 15u << word_shift(j);
+        if (mask != 0 && mask != 0xFFFFFFFFu)
+#pragma unroll
+            for (int i = 0; i < VW; i++) old[i] = vw[VW * threadIdx.x + i];
+    }
     const int x = threadIdx.x & 7;  // the lane's place in its block
     const int64_t row0 = (int64_t)e.first + p0 - from;
     for (int i = threadIdx.x >> 3; i < (hi - lo) * NB; i += 32) {
@@ -107,34 +140,39 @@ __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, c
         const float4 kx = *(const float4 *)(k + (row0 + p) * ldk + kvh * HD + 32 * blk + 4 * x);
         const float4 vx = *(const float4 *)(v + (row0 + p) * ldv + kvh * HD + 32 * blk + 4 * x);
         const uint16_t kd = kv4_scale(kx), vd = kv4_scale(vx);
-        const uint32_t kc = kv4_codes(kx, kd), vc = kv4_codes(vx, vd);
+        const uint32_t kc = kv4_codes(kx, kd), vcodes = kv4_codes(vx, vd);
         // codes of values 0..3 (even lane) or 4..7 (odd): nibbles 0, 4, 1, 5 or 2, 6, 3, 7
         uint32_t w = (kc & 15u) | (kc >> 8 & 15u) << 16 | (kc >> 16 & 15u) << 4 | (kc >> 24) << 20;
         w <<= 8 * (x & 1);
-        w |= __shfl_xor(w, 1, 64);
+        w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xB1, 0xF, 0xF, false);
         const int word = 4 * blk + (x >> 1), g = word / NB;
         if (!(x & 1)) kw[(((p >> 4) * 4 + g) * 16 + (p & 15)) * NB + word - g * NB] = w;
-        *(uint32_t *)&lv[p][32 * blk + 4 * x] = vc;
+        uint8_t *to = &lv[p][4 * (x & 3) * M + 2 * blk + (x >> 2)];
+#pragma unroll
+        for (int y = 0; y < 4; y++) to[y * M] = (uint8_t)(vcodes >> (8 * y));
         if (x == 0) {
             ks[32 * blk + 2 * (p & 15) + (p >> 4)] = kd;
             vs[32 * blk + 8 * ((p & 15) >> 2) + 4 * (p >> 4) + (p & 3)] = vd;
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < VWords<NB>::N; i += 256) {
-        int m, g, r;
-        VWords<NB>::at(i, m, g, r);
-        uint32_t w = 0, mask = 0;
+    if (mask == 0) return;
+    uint32_t q[8];  // the codes of position j, dim i in byte i (of positions outside the batch: any four bits)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int p = v_pos(g, j);
-            if (p < lo || p >= hi) continue;
-            w |= (uint32_t)lv[p][16 * m + r] << word_shift(j);
-            mask |= 15u << word_shift(j);
-        }
-        if (mask == 0xFFFFFFFFu) vw[i] = w;
-        else if (mask) vw[i] = (vw[i] & ~mask) | w;
+    for (int j = 0; j < 8; j++) {
+        const uint8_t *at = &lv[v_pos(vg, j)][vr * M + VW * vc];
+        q[j] = (VW == 4 ? *(const uint32_t *)at : *(const uint16_t *)at) & 0x0F0F0F0Fu;
     }
+    // nibbles 0 and 1, 2 and 3, 4 and 5, 6 and 7 of the words: positions 0 2, 4 6, 1 3, 5 7
+    const uint32_t n0 = q[0] | q[2] << 4, n1 = q[4] | q[6] << 4, n2 = q[1] | q[3] << 4, n3 = q[5] | q[7] << 4;
+#pragma unroll
+    for (int i = 0; i < VW; i++) {
+        const uint32_t w = (n0 >> (8 * i) & 255u) | (n1 >> (8 * i) & 255u) << 8 | (n2 >> (8 * i) & 255u) << 16 |
+                           (n3 >> (8 * i) & 255u) << 24;
+        old[i] = (old[i] & ~mask) | (w & mask);
+    }
+    if constexpr (VW == 4) *(uint4 *)(vw + 4 * threadIdx.x) = make_uint4(old[0], old[1], old[2], old[3]);
+    else *(uint2 *)(vw + 2 * threadIdx.x) = make_uint2(old[0], old[1]);
 }
 
 // ---- read ---------------------------------------------------------------------------------
