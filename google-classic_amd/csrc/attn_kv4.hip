@@ -99,6 +99,13 @@ struct Kv4Attn {
     int ctiles;  // tiles of 16 columns that max_rows rows have
 };
 
+// The partial sums of an entry's row and head, range after range: hd sums, the
+// maximum they are relative to and the probabilities' sum.
+__device__ __forceinline__ float *partial(const Kv4Attn &a, int entry, int row, int h, int hd)
+{
+    return a.part + ((((int64_t)entry * a.b.max_rows + row) * a.n_heads + h) * a.splits) * (hd + 4);
+}
+
 // Column c of an entry and KV head: row c / G, query head kvh * G + c % G.
 // Waves: W; the columns of a workgroup: 16.
 template <int NB, int W>
@@ -335,7 +342,7 @@ __global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
             if (too_long) y = f4{NAN, NAN, NAN, NAN};
             *(f4 *)(a.out + at * a.ldo + (int64_t)h * HD + d) = y;
         } else {
-            float *pp = a.part + ((at * a.n_heads + h) * a.splits + blockIdx.x) * (HD + 4);
+            float *pp = partial(a, blockIdx.z, (c0 + c) / G, h, HD) + (int64_t)blockIdx.x * (HD + 4);
             *(f4 *)(pp + d) = O;
             if (d == 0) *(f2 *)(pp + HD) = f2{M, L};
         }
@@ -360,7 +367,7 @@ __global__ __launch_bounds__(256) void attn_kv4_join_k(Kv4Attn a)
     const int n = (ntiles + a.chunk - 1) / a.chunk;
     if (n <= 1) return;
     const int64_t at = e.first + row;
-    const float *pp = a.part + ((at * a.n_heads + h) * a.splits) * (HD + 4);
+    const float *pp = partial(a, blockIdx.z, row, h, HD);
     const int g = threadIdx.x / D, d = 4 * (threadIdx.x % D);
     float M = -FLT_MAX, L = 0.f;
     f4 O = f4{};
@@ -435,18 +442,13 @@ static int run_attn(Kv4Attn a)
     a.splits = max(1, (tiles + a.chunk - 1) / a.chunk);
     const dim3 grid(a.splits, a.ctiles * a.c.n_kv_heads, a.b.n_seqs);
     constexpr size_t lds = (size_t)W * 16 * (32 * NB + 4 + 2) * sizeof(float);
-    static bool attr = false;
-    if (!attr) {
-        HOLO_CHECK(hipFuncSetAttribute((const void *)attn_kv4_k<NB, W>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)lds));
-        attr = true;
-    }
     if (a.splits == 1) {
         hipLaunchKernelGGL((attn_kv4_k<NB, W>), grid, dim3(64 * W), lds, stream(), a);
         HOLO_LAUNCH_CHECK();
         return 0;
     }
-    const StreamScratch scratch((size_t)a.b.rows * a.n_heads * a.splits * (32 * NB + 4) * sizeof(float));
+    // (a small buffer: ranges are for fewer than two workgroups a CU, and make fewer than four)
+    const StreamScratch scratch((size_t)a.b.n_seqs * take * a.n_heads * a.splits * (32 * NB + 4) * sizeof(float));
     a.part = (float *)scratch.get();
     if (!a.part) {
         latch_error((int)hipErrorOutOfMemory, "holo_attention_kv4: partial sums", __FILE__, __LINE__);

@@ -114,6 +114,7 @@ __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, c
     __shared__ __align__(16) uint8_t lv[32][HD];  // [position][16 r's][M dims r + 16 m]
     const Kv4Entry e = kv4_entry(c, b, blockIdx.z);
     const int kvh = blockIdx.y, from = e.len - e.rows;  // position of the entry's first row
+    if ((int)blockIdx.x > (e.take + 30) / 32) return;  // (so that 32 t stays an int)
     const int t = (max(from, 0) >> 5) + blockIdx.x, p0 = 32 * t;
     // the tile's positions in the batch: lo .. hi - 1
     const int lo = max(from - p0, 0), hi = min(min(from + e.take, e.len) - p0, 32);
@@ -186,6 +187,7 @@ __global__ __launch_bounds__(256) void kv4_read_k(Kv4View c, holo_batch_t b, flo
     const int kvh = blockIdx.y, from = e.len - e.rows;
     // rows before position 0 and of a tile without a page are zeros: the tiles are
     // counted from the one of `from`, which may be negative
+    if ((int)blockIdx.x > (e.take + 30) / 32) return;
     const int t = (from >> 5) + (int)blockIdx.x, p0 = 32 * t;
     const int lo = max(from - p0, 0), hi = min(from + e.take - p0, 32);
     if (lo >= hi) return;
@@ -291,7 +293,7 @@ bool kv4_layout_ok(const holo_kv4_t *c)
 
 bool batch_ok(const holo_batch_t *b)
 {
-    return b && b->rows >= 0 && b->n_seqs >= 0 && b->n_seqs <= 65535 &&
+    return b && b->rows >= 0 && b->rows <= 0x7FFFF000 && b->n_seqs >= 0 && b->n_seqs <= 65535 &&
            (b->rows == 0 || b->n_seqs == 0 || (b->cu_rows && b->max_rows > 0));
 }
 

@@ -420,3 +420,95 @@ def test_copies_of_pages(holo):
         holo.check("copy")
         c.pool[dst] = c.pool[src]
         assert np.array_equal(dev.bytes(), c.pool)
+
+
+def test_pool_past_four_gigabytes(holo):
+    """Pages whose bytes lie past 2^32, written, read, attended and copied from."""
+    print("case kv4 large pool", flush=True)
+    rng = np.random.default_rng(11)
+    hd, heads, n_kv, n, layer = 128, 8, 8, 1500, 7
+    c = Cache(hd, 1024, 1, n_kv, 1, 1, 2, fill=0)  # the arrays around a pool that only the device holds
+    dev, lib = OnDevice(holo, c), holo.lib()
+    dev.desc.n_layers, dev.desc.n_pages = 8, 500
+    size = lib.holo_kv4_page_bytes(dev.ref)
+    assert 470 * size > 1 << 32
+    dev.pool = holo.DeviceBuffer(500 * size)
+    dev.desc.pool = dev.pool.ptr
+    c.table[0], c.len[0] = (499, 470), n
+    dev.refresh()
+    k, v = rng.standard_normal((2, n, n_kv * hd)).astype(np.float32)
+    q = rng.standard_normal((3, heads * hd)).astype(np.float32)
+    dk, dv, dq, do = up(holo, k), up(holo, v), up(holo, q), holo.DeviceBuffer(q.nbytes)
+    b = Batch(holo, [n], None, None, n)
+    assert lib.holo_kv4_append(dev.ref, layer, dk.ptr, dv.ptr, n_kv * hd, n_kv * hd, b.ref) == 0
+    hk, hv = values(*quantise(k)), values(*quantise(v))
+    last = Batch(holo, [3], None, None, n)
+    for pages_ in ((499, 470), (3, 498)):
+        c.table[0] = pages_
+        dev.refresh()
+        if pages_[0] == 3:
+            src, dst = np.int32([470, 499]), np.int32([498, 3])
+            assert lib.holo_kv4_copy_pages(dev.ref, src.ctypes.data, dst.ctypes.data, 2) == 0
+        dk.upload(np.zeros_like(k))
+        assert lib.holo_kv4_read(dev.ref, layer, dk.ptr, dv.ptr, n_kv * hd, n_kv * hd, b.ref) == 0
+        assert lib.holo_attention_kv4(dev.ref, layer, do.ptr, dq.ptr, heads * hd, heads * hd, heads, last.ref) == 0
+        lib.cuda_sync()
+        holo.check("large pool")
+        assert np.array_equal(dk.download(np.float32).reshape(n, -1), hk)
+        assert np.array_equal(dv.download(np.float32).reshape(n, -1), hv)
+        got, want = do.download(np.float32).reshape(3, heads, hd), np.zeros((3, heads, hd))
+        for i in range(3):
+            for h in range(heads):
+                x = slice(h * hd, (h + 1) * hd)
+                s = hk[:n - 2 + i, x] @ q[i, x].astype(np.float64) / np.sqrt(hd)
+                p = np.exp(s - s.max())
+                want[i, h] = p / p.sum() @ hv[:n - 2 + i, x]
+        assert normwise(got, want) <= TOL
+
+
+def test_the_last_positions_there_are(holo):
+    """A sequence of 0x7FFFF000 positions, of which the last pages are there."""
+    print("case kv4 last positions", flush=True)
+    rng = np.random.default_rng(12)
+    hd, rows, n = 32, 70, 0x7FFFF000
+    c = Cache(hd, 1024, 1, 1, 2, 1, n // 1024, fill=0x30)  # scales of 0x3030: 7 significant bits
+    c.table[0, -1], c.len[0] = 1, n
+    dev, lib = OnDevice(holo, c), holo.lib()
+    k, v, q = rng.standard_normal((3, rows, hd)).astype(np.float32)
+    dk, dv, dq, do = up(holo, k), up(holo, v), up(holo, q), holo.DeviceBuffer(q.nbytes)
+    b = Batch(holo, [rows], None, None, n)
+    b.desc.max_rows = b.desc.rows = 0x7FFFF000  # bounds: the entry has 70
+    assert lib.holo_kv4_append(dev.ref, 0, dk.ptr, dv.ptr, hd, hd, b.ref) == 0
+    assert lib.holo_kv4_read(dev.ref, 0, dk.ptr, dv.ptr, hd, hd, b.ref) == 0
+    b.desc.max_rows = 1  # and one of them here
+    assert lib.holo_attention_kv4(dev.ref, 0, do.ptr, dq.ptr, hd, hd, 1, b.ref) == 0
+    lib.cuda_sync()
+    holo.check("last positions")
+    assert np.array_equal(dk.download(np.float32).reshape(rows, hd), values(*quantise(k)))
+    assert np.array_equal(dv.download(np.float32).reshape(rows, hd), values(*quantise(v)))
+    held = [np.stack([c.get(0, 0, 0, p, w) for p in range(n - 1024, n - rows)]) for w in (0, 1)]
+    hk, hv = (np.concatenate([x, values(*quantise(y))[:1]]) for x, y in zip(held, (k, v)))
+    s = hk @ q[0].astype(np.float64) / np.sqrt(hd)
+    p = np.exp(s - s.max())
+    assert normwise(do.download(np.float32)[:hd], p / p.sum() @ hv) <= TOL
+
+
+@pytest.mark.parametrize("scale", [1e12, 1e20, 1e30, -1e25])
+def test_scores_far_past_the_exponential(holo, scale):
+    """Scores so large that one position has all of the probability: its value comes back."""
+    print(f"case kv4 scale {scale}", flush=True)
+    rng = np.random.default_rng(13)
+    hd, heads, n_kv, n = 64, 4, 2, 800
+    c = Cache(hd, 64, 1, n_kv, 13, 1, 13)
+    pages(c, [n], rng)
+    fill(c, rng, [n], 0)
+    q = (scale * rng.standard_normal((1, heads * hd))).astype(np.float32)
+    got = attention(holo, OnDevice(holo, c), 0, q, [1], heads).reshape(heads, hd)
+    for h in range(heads):
+        k, v, _ = c.held(0, 0, h // 2, n)
+        s = k @ q[0, h * hd:(h + 1) * hd].astype(np.float64)
+        first, second = np.sort(s)[::-1][:2]
+        # a score is within 9.5e-7 of the sum of magnitudes, about 4e-6 of the largest
+        assert first - second > 1e-4 * first
+        # p is 2^7.5 in two halves, and its sum the same number
+        assert np.abs(got[h] - v[s.argmax()]).max() <= 2.0 ** -21 * np.abs(v[s.argmax()]).max()
