@@ -16,10 +16,13 @@
 //     they stand.  Pieces are permuted (XOR) so that the writes and the reads of 16
 //     lanes fall on 64 different banks.
 //   - Keys and values are held times 2^8, which suits f16 for rows whose largest
-//     value is in [2^-11, 2^8); q rows are scaled to their largest value.  Where
-//     the keys that a workgroup walks hold any other row (or an infinity or NaN,
-//     which the matrix instructions would hand to the rows that do not see it), it
-//     starts over in fp32, value by value: right for anything, and slow.
+//     value is in [2^-11, 2^8); q rows are scaled to their largest value.  Smaller
+//     rows are held within 2^-33, which does no harm to scores of ordinary q rows, nor
+//     to outputs that other rows have a part in.  The columns that it harms, and
+//     every column of a workgroup that walks a row of larger values (or of infinities
+//     or NaN, which the matrix instructions would hand to the rows that do not see
+//     it), start over in fp32, value by value: right for anything, and slow (1024
+//     rows with two small ones 68 us, as without them; 4096 with one of 300: 11.7 ms).
 //   - The softmax is one pass; the running maximum moves only when a score passes
 //     it by 2^7 (attn_tiles.h).
 // KV heads are the fastest grid index, so that with 8 of them each XCD's L2 holds
@@ -47,6 +50,12 @@ struct PackedAttn {
 
 constexpr float kHeld = 256.f;                               // keys and values are held times this
 constexpr float kRowLow = 1.f / 2048.f, kRowHigh = 256.f;    // a row's largest value
+// What a workgroup's staged rows hold that the halves do not suit.  Low rows are
+// held within 2^-33: no harm to a column whose scores that moves by 2^-22 at most (hd
+// values of q below 16 in log2 units, sc below kLowSc), or whose output's
+// largest value is not low itself.
+enum { kHighRow = 1, kLowKey = 2, kLowValue = 4 };
+constexpr float kLowSc = 0x1p-17f;
 
 // The largest magnitude of four values; NaN if one is.
 __device__ __forceinline__ float most(const f4 x)
@@ -90,10 +99,11 @@ struct PackedLds {
     static constexpr int HD = 32 * NB;  // HD / 8 <= 16
     // [hi, lo][dims 8 d8 ..][key ^ (d8 & 15)] and [hi, lo][dims 32 b ..][keys' group][dim]
     h8 k[2][2][HD / 8][32], v[2][2][NB][4][32];
-    int odd[8];  // by wave: a staged row that the halves do not suit
+    int odd[8];  // by wave: of the rows that it staged
 };
 
-// One column in fp32 by the two lanes that hold it, half of the dims each.
+// One column in fp32 by the two lanes that hold it, half of the dims each, four
+// keys at a time.
 template <int HD>
 __device__ __forceinline__ void packed_fp32(const PackedAttn &a, const float *qp, const float *kb, const float *vb,
                                             int row, int hh, float *out)
@@ -105,22 +115,48 @@ __device__ __forceinline__ void packed_fp32(const PackedAttn &a, const float *qp
 #pragma unroll
     for (int i = 0; i < H / 4; i++) o[i] = f4{};
     qp += H * hh, kb += H * hh, vb += H * hh, out += H * hh;
-    for (int key = 0; key <= row; key++) {
-        const f4 *k = (const f4 *)(kb + (int64_t)key * a.ldk), *v = (const f4 *)(vb + (int64_t)key * a.ldv);
-        f4 d4 = f4{};
-#pragma unroll 4
-        for (int i = 0; i < H / 4; i++) d4 += ((const f4 *)qp)[i] * k[i];
-        float s = (d4[0] + d4[1]) + (d4[2] + d4[3]);
-        s = (s + __shfl_xor(s, 32, 64)) * score_scale(HD);
-        const float mx = fmaxf(m, s), w = __builtin_amdgcn_exp2f(m - mx), p = __builtin_amdgcn_exp2f(s - mx);
-        m = mx;
-        // the average so far: a sum of values next to the largest float would overflow
-        const float was = l * w;
-        l = was + p;
-        const float keep = was / l, add = p / l;
+    auto keys = [&]<int N>(int key) {
+        f4 d[N];
+        float s[N], mx = m;
 #pragma unroll
-        for (int i = 0; i < H / 4; i++) o[i] = o[i] * keep + add * v[i];
-    }
+        for (int n = 0; n < N; n++) d[n] = f4{};
+        const float *k = kb + (int64_t)key * a.ldk, *v = vb + (int64_t)key * a.ldv;
+#pragma unroll 4
+        for (int i = 0; i < H / 4; i++) {
+            const f4 x = ((const f4 *)qp)[i];
+#pragma unroll
+            for (int n = 0; n < N; n++)
+                d[n] = __builtin_elementwise_fma(x, ((const f4 *)(k + (int64_t)n * a.ldk))[i], d[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            s[n] = (d[n][0] + d[n][1]) + (d[n][2] + d[n][3]);
+            s[n] = (s[n] + __shfl_xor(s[n], 32, 64)) * score_scale(HD);
+            mx = fmaxf(mx, s[n]);
+        }
+        // the average so far: a sum of values next to the largest float would overflow
+        const float was = l * __builtin_amdgcn_exp2f(m - mx);
+        m = mx;
+        l = was;
+#pragma unroll
+        for (int n = 0; n < N; n++) l += s[n] = __builtin_amdgcn_exp2f(s[n] - mx);
+        const float keep = was / l;
+#pragma unroll
+        for (int n = 0; n < N; n++) s[n] /= l;
+#pragma unroll
+        for (int i = 0; i < H / 4; i++) {
+            f4 y = o[i] * keep;
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                const f4 x = ((const f4 *)(v + (int64_t)n * a.ldv))[i];
+                y = __builtin_elementwise_fma(f4{s[n], s[n], s[n], s[n]}, x, y);
+            }
+            o[i] = y;
+        }
+    };
+    int key = 0;
+    for (; key + 3 <= row; key += 4) keys.template operator()<4>(key);
+    for (; key <= row; key++) keys.template operator()<1>(key);
 #pragma unroll
     for (int i = 0; i < H / 4; i++) ((f4 *)out)[i] = o[i];
 }
@@ -213,19 +249,19 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
             }
         }
     };
-    // whether the loaded rows suit the halves
-    bool odd = false;
-    auto check = [&]() {
+    // whether the loaded rows suit the halves; low: kLowKey or kLowValue
+    int odd = 0;
+    auto check = [&](int low) {
         float big = 0.f, m[KP];
 #pragma unroll
         for (int i = 0; i < KP; i++) {
             m[i] = most(ld[i]);
             big = __builtin_elementwise_maximum(big, m[i]);
         }
-        odd |= __any(!(big < kRowHigh));
+        odd |= __any(!(big < kRowHigh)) ? kHighRow : 0;
         if (some_low<LPR>(m)) {  // a row of small values, or of zeros
 #pragma unroll
-            for (int i = 0; i < KP; i++) odd |= low_row<LPR>(m[i]);
+            for (int i = 0; i < KP; i++) odd |= low_row<LPR>(m[i]) ? low : 0;
         }
     };
     const bool second = W == 8 && wave >= 4;
@@ -256,7 +292,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
         }
         sc = ldexpf(1.f / kHeld, ex);
     }
-    check();
+    check(second ? kLowValue : kLowKey);
     if (second) {
 #pragma unroll
         for (int i = 0; i < 4; i++) store_v(0, i);
@@ -266,7 +302,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
         for (int i = 0; i < KP; i++) store_k(0, i);
         if constexpr (W == 4) {
             load_v(0);
-            check();
+            check(kLowValue);
 #pragma unroll
             for (int i = 0; i < 4; i++) store_v(0, i);
         }
@@ -376,7 +412,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
             scores(b, [&](int c) {
                 // the next tile's keys into LDS, once their loads are there
                 constexpr int H = NC / 2;
-                if (c == H) check();
+                if (c == H) check(kLowKey);
 #pragma unroll
                 for (int i = KP * (c - H) / H; c >= H && i < KP * (c - H + 1) / H; i++) store_k(b ^ 1, i);
             });
@@ -389,7 +425,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
                 read_v(b, 0);
                 probabilities();
                 values(b, [&](int x) {
-                    if (x == NB) check();
+                    if (x == NB) check(kLowValue);
 #pragma unroll
                     for (int d = 4 * (x - NB) / NB; x >= NB && d < 4 * (x - NB + 1) / NB; d++) store_v(b ^ 1, d);
                 });
@@ -408,7 +444,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
             for (; t < ntiles && !moves(t); t++) {
                 const int b = t & 1;
                 probabilities();
-                check();
+                check(second ? kLowValue : kLowKey);
                 if (second) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) store_v(b ^ 1, i);
@@ -431,25 +467,34 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
         }
         if (!second) __syncthreads();
     }
-    // rows that the halves do not suit: over again
+    // columns that the halves do not suit: over again
     if (lane == 0) S.odd[wave] = odd;
     __syncthreads();
-    bool over = false;
+    odd = 0;
 #pragma unroll
-    for (int w = 0; w < W; w++) over |= S.odd[w] != 0;
+    for (int w = 0; w < W; w++) odd |= S.odd[w];
+    l += __shfl_xor(l, 32, 64);
+    const float f = 1.0f / (kHeld * l);  // a row sees itself
+    bool over = odd & kHighRow || (odd & kLowKey && sc >= kLowSc);
+    if (odd & kLowValue) {
+        float big = 0.f;
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) big = fmaxf(big, fabsf(o[i][r]));
+        over |= max_halves(big) * f < kRowLow;
+    }
+    if (w0 + j >= ncols) return;
+    float *op = a.out + (int64_t)(s0 + row) * a.ldo + (int64_t)head * HD;
     if (over) {
-        if (w0 + j < ncols) packed_fp32<HD>(a, qp, kb, vb, row, hh, a.out + (int64_t)(s0 + row) * a.ldo + (int64_t)head * HD);
+        packed_fp32<HD>(a, qp, kb, vb, row, hh, op);
         return;
     }
-    l += __shfl_xor(l, 32, 64);
-    if (w0 + j >= ncols) return;
-    const float f = 1.0f / (kHeld * l);  // a row sees itself
-    float *op = a.out + (int64_t)(s0 + row) * a.ldo + (int64_t)head * HD + 4 * hh;
 #pragma unroll
     for (int i = 0; i < NB; i++)
 #pragma unroll
         for (int r = 0; r < 16; r += 4)
-            *(f4 *)(op + 32 * i + 2 * r) = f4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]} * f;
+            *(f4 *)(op + 4 * hh + 32 * i + 2 * r) = f4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]} * f;
 }
 
 // ---- few columns: the keys shared by the waves ----------------------------------------
@@ -575,7 +620,7 @@ __global__ __launch_bounds__(64 * W, 8 / W) void attn_packed_split_k(PackedAttn 
     const float *const kget = &S.k[wave][j][8 * hh];
 
     float m = -FLT_MAX, l = 0.f;
-    bool odd = false;
+    int odd = 0;
     f16v o[NB];
 #pragma unroll
     for (int i = 0; i < NB; i++) o[i] = f16v{};
@@ -598,12 +643,12 @@ __global__ __launch_bounds__(64 * W, 8 / W) void attn_packed_split_k(PackedAttn 
                 for (int i = 1; i < NB; i++) mv[r] = __builtin_elementwise_maximum(mv[r], fabsf(vr[r][i]));
                 big = __builtin_elementwise_maximum(big, mv[r]);
             }
-            odd |= __any(!(big < kRowHigh));
+            odd |= __any(!(big < kRowHigh)) ? kHighRow : 0;
             if (some_low<LR>(mk) || some_low<32>(mv)) {
 #pragma unroll
-                for (int i = 0; i < NI; i++) odd |= low_row<LR>(mk[i]);
+                for (int i = 0; i < NI; i++) odd |= low_row<LR>(mk[i]) ? kLowKey : 0;
 #pragma unroll
-                for (int r = 0; r < 16; r++) odd |= low_row<32>(mv[r]);
+                for (int r = 0; r < 16; r++) odd |= low_row<32>(mv[r]) ? kLowValue : 0;
             }
         }
         f16v s = f16v{};
@@ -684,14 +729,6 @@ __global__ __launch_bounds__(64 * W, 8 / W) void attn_packed_split_k(PackedAttn 
     }
     if (lane == 0) S.odd[wave] = odd;
     __syncthreads();
-    bool over = false;
-#pragma unroll
-    for (int w = 0; w < W; w++) over |= S.odd[w] != 0;
-    if (over) {
-        if (wave == 0 && c0 + j < ncols)
-            packed_fp32<HD>(a, qp, kb, vb, row, hh, a.out + (int64_t)(s0 + row) * a.ldo + (int64_t)head * HD);
-        return;
-    }
     if (threadIdx.x < 32) {
         float M = S.m[0][j], L = 0.f;
 #pragma unroll
@@ -705,14 +742,34 @@ __global__ __launch_bounds__(64 * W, 8 / W) void attn_packed_split_k(PackedAttn 
 #pragma unroll
         for (int w = 0; w < W; w++) S.w[w][j] = f[w] / (kHeld * L);
     }
+    odd = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) odd |= S.odd[w];
     __syncthreads();
-    for (int e = threadIdx.x; e < 32 * HD; e += 64 * W) {
-        const int c = e / HD, d = e % HD;
-        if (c0 + c >= ncols) continue;
+    auto at = [&](int c, int d) {
         float O = 0.f;
 #pragma unroll
         for (int w = 0; w < W; w++) O = fmaf(S.w[w][c], S.o[w][c][d], O);
-        a.out[(int64_t)(s0 + (c0 + c) / G) * a.ldo + (int64_t)(kvh * G + (c0 + c) % G) * HD + d] = O;
+        return O;
+    };
+    if (odd) {  // columns that the halves do not suit: over again
+        if (wave == 0) {
+            bool over = odd & kHighRow || (odd & kLowKey && sc >= kLowSc);
+            if (odd & kLowValue) {
+                float big = 0.f;
+                for (int d = 0; d < HD / 2; d++) big = fmaxf(big, fabsf(at(j, HD / 2 * hh + d)));
+                over |= max_halves(big) < kRowLow;
+            }
+            if (hh == 0) S.m[0][j] = over ? 1.f : 0.f;
+            if (over && c0 + j < ncols)
+                packed_fp32<HD>(a, qp, kb, vb, row, hh, a.out + (int64_t)(s0 + row) * a.ldo + (int64_t)head * HD);
+        }
+        __syncthreads();
+    }
+    for (int e = threadIdx.x; e < 32 * HD; e += 64 * W) {
+        const int c = e / HD, d = e % HD;
+        if (c0 + c >= ncols || (odd && S.m[0][c] != 0.f)) continue;
+        a.out[(int64_t)(s0 + (c0 + c) / G) * a.ldo + (int64_t)(kvh * G + (c0 + c) % G) * HD + d] = at(c, d);
     }
 }
 

@@ -199,3 +199,40 @@ def test_captured(holo):
     finally:
         lib.holo_set_stream(before)
         lib.holo_stream_destroy(st)
+
+
+@pytest.mark.parametrize("hd,heads,n_kv,rows", [
+    (64, 4, 2, [100]), (96, 4, 2, [20, 30]), (128, 64, 64, [1030]), (128, 16, 4, [600]), (32, 8, 8, [40] * 200),
+], ids=str)
+@pytest.mark.parametrize("low,sq", [(1e-5, 1), (1e-12, 1), (1e-5, 30)])
+def test_low_rows_among_others(holo, hd, heads, n_kv, rows, low, sq):
+    """Keys and values far smaller than their neighbours': a sequence's first rows
+    (which rows see alone, and with others), and one in the middle that a head's rows look at
+    alone.  Each row and head by itself, within what its scores allow."""
+    print(f"case packed low rows hd {hd} heads {heads}/{n_kv} rows {rows[:3]} {low} {sq}", flush=True)
+    total = sum(rows)
+    q, k, v = inputs(8, total, hd, heads, n_kv)
+    q *= np.float32(sq)
+    at = 0
+    for n in rows:
+        k[at:at + 3] *= np.float32(low)
+        v[at:at + 3] *= np.float32(low)
+        v[at + n // 2] *= np.float32(low)
+        k[at + n // 2, :hd] = np.sign(q[at + n - 1, :hd])  # the last row's first head
+        at += n
+    got, at = run(holo, q, k, v, rows, hd, heads, n_kv), 0
+    for n in rows[:2]:
+        for h in (0, heads - 1):
+            g = h * n_kv // heads
+            kh, vh = (x[at:at + n, g * hd:(g + 1) * hd].astype(np.float64) for x in (k, v))
+            s = q[at:at + n, h * hd:(h + 1) * hd].astype(np.float64) @ kh.T / np.sqrt(hd)
+            s[np.arange(n)[None] > np.arange(n)[:, None]] = -np.inf
+            p = np.exp(s - s.max(1, keepdims=True))
+            want = (p / p.sum(1, keepdims=True)) @ vh
+            x = got[at:at + n, h * hd:(h + 1) * hd]
+            err = np.linalg.norm(x - want, axis=1) / np.linalg.norm(want, axis=1)
+            # a score is within 1.2e-5 of it at most for q of about 1, and a row's average within that of
+            # the values that it averages, which cancel up to 1 / sqrt(n)
+            assert err.max() <= 1.2e-5 * sq * np.sqrt(n)
+            assert np.median(err) <= TOL * sq
+        at += n
