@@ -249,19 +249,19 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
             }
         }
     };
-    // whether the loaded rows suit the halves; low: kLowKey or kLowValue
-    int odd = 0;
-    auto check = [&](int low) {
+    // whether the loaded rows suit the halves; low: of the keys', or of the values
+    bool high = false, low_k = false, low_v = false;
+    auto check = [&](bool &low) {
         float big = 0.f, m[KP];
 #pragma unroll
         for (int i = 0; i < KP; i++) {
             m[i] = most(ld[i]);
             big = __builtin_elementwise_maximum(big, m[i]);
         }
-        odd |= __any(!(big < kRowHigh)) ? kHighRow : 0;
+        high |= __any(!(big < kRowHigh));
         if (some_low<LPR>(m)) {  // a row of small values, or of zeros
 #pragma unroll
-            for (int i = 0; i < KP; i++) odd |= low_row<LPR>(m[i]) ? low : 0;
+            for (int i = 0; i < KP; i++) low |= low_row<LPR>(m[i]);
         }
     };
     const bool second = W == 8 && wave >= 4;
@@ -292,7 +292,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
         }
         sc = ldexpf(1.f / kHeld, ex);
     }
-    check(second ? kLowValue : kLowKey);
+    check(low_k);
     if (second) {
 #pragma unroll
         for (int i = 0; i < 4; i++) store_v(0, i);
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
         for (int i = 0; i < KP; i++) store_k(0, i);
         if constexpr (W == 4) {
             load_v(0);
-            check(kLowValue);
+            check(low_v);
 #pragma unroll
             for (int i = 0; i < 4; i++) store_v(0, i);
         }
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
             scores(b, [&](int c) {
                 // the next tile's keys into LDS, once their loads are there
                 constexpr int H = NC / 2;
-                if (c == H) check(kLowKey);
+                if (c == H) check(low_k);
 #pragma unroll
                 for (int i = KP * (c - H) / H; c >= H && i < KP * (c - H + 1) / H; i++) store_k(b ^ 1, i);
             });
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
                 read_v(b, 0);
                 probabilities();
                 values(b, [&](int x) {
-                    if (x == NB) check(kLowValue);
+                    if (x == NB) check(low_v);
 #pragma unroll
                     for (int d = 4 * (x - NB) / NB; x >= NB && d < 4 * (x - NB + 1) / NB; d++) store_v(b ^ 1, d);
                 });
@@ -444,7 +444,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
             for (; t < ntiles && !moves(t); t++) {
                 const int b = t & 1;
                 probabilities();
-                check(second ? kLowValue : kLowKey);
+                check(low_k);  // (of the values, in the second group)
                 if (second) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) store_v(b ^ 1, i);
@@ -468,9 +468,10 @@ __global__ __launch_bounds__(64 * W, 2) void attn_packed_k(PackedAttn a)
         if (!second) __syncthreads();
     }
     // columns that the halves do not suit: over again
-    if (lane == 0) S.odd[wave] = odd;
+    if (second) low_v = low_k, low_k = false;
+    if (lane == 0) S.odd[wave] = (high ? kHighRow : 0) | (low_k ? kLowKey : 0) | (low_v ? kLowValue : 0);
     __syncthreads();
-    odd = 0;
+    int odd = 0;
 #pragma unroll
     for (int w = 0; w < W; w++) odd |= S.odd[w];
     l += __shfl_xor(l, 32, 64);
