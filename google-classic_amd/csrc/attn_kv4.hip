@@ -37,8 +37,7 @@ __device__ __forceinline__ h8 kv4_unpack(uint32_t w, uint32_t k16, const h2 d[4]
     h2 x[4];
 #pragma unroll
     for (int p = 0; p < 4; p++) {
-        // (of a word as stored: value pair p at bits 4 p + 2)
-        const uint32_t n = p == 0 ? w << 4 : p == 1 ? w : p == 2 ? w >> 4 : __builtin_rotateright32(w, 8);
+        const uint32_t n = p < 2 ? w << (6 - 4 * p) : w >> (4 * p - 6);
         x[p] = __builtin_elementwise_fma(__builtin_bit_cast(h2, (n & 0x03C003C0u) | k16), d[p], d24[p]);
     }
     return h8{x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};

@@ -12,9 +12,8 @@
 //      holds after the first product, so that the probabilities are the second
 //      one's B operand as they stand;
 //   scales: K [block][r][half], V [block][g][8], f16.
-// Value i of a word is nibble i / 2 + 4 (i % 2) of the word turned right by two
-// bits: a shift (none for values 2 and 3) and a mask bring values 2 p and 2 p + 1
-// to bits 6 .. 9 of a register's halves.
+// Value i of a word is nibble i / 2 + 4 (i % 2): a shift and a mask bring values
+// 2 p and 2 p + 1 into the halves of a register.
 #pragma once
 
 #include "common.h"
@@ -62,10 +61,7 @@ __device__ __forceinline__ uint8_t *kv4_tile(const Kv4View &c, const Kv4Entry &e
     return c.pool + at * (36 * 32 * NB);
 }
 
-__device__ __forceinline__ uint32_t word_in(uint32_t w) { return __builtin_rotateright32(w, 2); }
-__device__ __forceinline__ uint32_t word_out(uint32_t w) { return __builtin_rotateleft32(w, 2); }
-
-// Position of value i of lane group g's V words, and the bit of value i of a word turned in.
+// Position of value i of lane group g's V words, and the bit of a word's value i.
 __device__ __forceinline__ int v_pos(int g, int i) { return i < 4 ? 4 * g + i : 12 + 4 * g + i; }
 __device__ __forceinline__ int word_shift(int i) { return 4 * (i >> 1) + 16 * (i & 1); }
 

@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, c
             if (v_pos(vg, j) >= lo && v_pos(vg, j) < hi) mask |= 15u << word_shift(j);
         if (mask != 0 && mask != 0xFFFFFFFFu)
 #pragma unroll
-            for (int i = 0; i < VW; i++) old[i] = word_in(vw[VW * threadIdx.x + i]);
+            for (int i = 0; i < VW; i++) old[i] = vw[VW * threadIdx.x + i];
     }
     const int x = threadIdx.x & 7;  // the lane's place in its block
     const int64_t row0 = (int64_t)e.first + p0 - from;
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, c
         w <<= 8 * (x & 1);
         w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xB1, 0xF, 0xF, false);
         const int word = 4 * blk + (x >> 1), g = word / NB;
-        if (!(x & 1)) kw[(((p >> 4) * 4 + g) * 16 + (p & 15)) * NB + word - g * NB] = word_out(w);
+        if (!(x & 1)) kw[(((p >> 4) * 4 + g) * 16 + (p & 15)) * NB + word - g * NB] = w;
         uint8_t *to = &lv[p][4 * (x & 3) * M + 2 * blk + (x >> 2)];
 #pragma unroll
         for (int y = 0; y < 4; y++) to[y * M] = (uint8_t)(vcodes >> (8 * y));
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, c
     for (int i = 0; i < VW; i++) {
         const uint32_t w = (n0 >> (8 * i) & 255u) | (n1 >> (8 * i) & 255u) << 8 | (n2 >> (8 * i) & 255u) << 16 |
                            (n3 >> (8 * i) & 255u) << 24;
-        old[i] = word_out((old[i] & ~mask) | (w & mask));
+        old[i] = (old[i] & ~mask) | (w & mask);
     }
     if constexpr (VW == 4) *(uint4 *)(vw + 4 * threadIdx.x) = make_uint4(old[0], old[1], old[2], old[3]);
     else *(uint2 *)(vw + 2 * threadIdx.x) = make_uint2(old[0], old[1]);
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256) void kv4_read_k(Kv4View c, holo_batch_t b, flo
         for (int i = threadIdx.x; i < VWords<NB>::N; i += 256) {
             int m, g, r;
             VWords<NB>::at(i, m, g, r);
-            const uint32_t w = word_in(vw[i]);
+            const uint32_t w = vw[i];
 #pragma unroll
             for (int j = 0; j < 8; j++) lv[v_pos(g, j)][16 * m + r] = (uint8_t)(w >> word_shift(j) & 15u);
         }
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256) void kv4_read_k(Kv4View c, holo_batch_t b, flo
             const float kd = (float)ks[32 * blk + 2 * (p & 15) + (p >> 4)];
             const float vd = (float)vs[32 * blk + 8 * ((p & 15) >> 2) + 4 * (p >> 4) + (p & 3)];
             const int word = 4 * blk + (x >> 1), g = word / NB;
-            const uint32_t w = word_in(kw[(((p >> 4) * 4 + g) * 16 + (p & 15)) * NB + word - g * NB]) >> (8 * (x & 1));
+            const uint32_t w = kw[(((p >> 4) * 4 + g) * 16 + (p & 15)) * NB + word - g * NB] >> (8 * (x & 1));
             const uint32_t vc = *(const uint32_t *)&lv[p][32 * blk + 4 * x];
             ko = make_float4(kd * (float)((int)(w & 15u) - 8), kd * (float)((int)(w >> 16 & 15u) - 8),
                              kd * (float)((int)(w >> 4 & 15u) - 8), kd * (float)((int)(w >> 20 & 15u) - 8));

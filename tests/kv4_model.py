@@ -131,21 +131,13 @@ def want_attention(cache, layer, q, rows, lens, seqs, n_heads):
     return out
 
 
-def turned(pool, hd, bits):
-    """The pool with its code words turned left by `bits`: the device's are, by two."""
-    out = pool.copy()
-    w = np.ascontiguousarray(pool[..., :32 * hd]).view(np.uint32)
-    out[..., :32 * hd] = ((w << np.uint32(bits)) | (w >> np.uint32(32 - bits))).view(np.uint8)
-    return out
-
-
 class OnDevice:
     """A Cache's arrays on the device, and its descriptor."""
 
     def __init__(self, holo, cache):
         self.holo, self.cache = holo, cache
         up = holo.DeviceBuffer.from_array
-        self.pool, self.table, self.len = up(turned(cache.pool, cache.hd, 2)), up(cache.table), up(cache.len)
+        self.pool, self.table, self.len = up(cache.pool), up(cache.table), up(cache.len)
         self.desc = holo.KV4(pool=self.pool.ptr, table=self.table.ptr, len=self.len.ptr, n_pages=cache.n_pages,
                              page_len=cache.page_len, n_layers=cache.n_layers, n_kv_heads=cache.n_kv,
                              head_dim=cache.hd, n_seqs=cache.n_seqs, max_pages=cache.max_pages)
@@ -156,7 +148,7 @@ class OnDevice:
         self.len.upload(self.cache.len)
 
     def bytes(self):
-        return turned(self.pool.download(np.uint8).reshape(self.cache.pool.shape), self.cache.hd, 30)
+        return self.pool.download(np.uint8).reshape(self.cache.pool.shape)
 
 
 class Batch:
