@@ -78,9 +78,12 @@ typedef struct {
  * (holo_attention_prefill at pos0 = 0, entry by entry).  ldo, ldq, ldk and ldv
  * are the floats from one row to the next (q, k and v may lie side by side in
  * one buffer).  head_dim 32, 64, 96 or 128; every pointer 16-byte aligned and
- * every ld a multiple of 4.  seqs and max_len are not read.  A row is not
- * touched by what the rows behind it hold, infinities and NaN among it.
- * Returns 0 or HOLO_EINVAL (nothing launched).                               */
+ * every ld a multiple of 4, ldk and ldv below 2^24; max_rows times n_heads /
+ * n_kv_heads up to 2097120.  seqs and max_len are not read.  A row is not
+ * touched by what the rows behind it hold, infinities and NaN among it.  Any
+ * magnitude is right; keys or values of 256 and more (and rows of which none
+ * reaches 2^-11, where they make up an output) take an fp32 path some thirty
+ * times slower.  Returns 0 or HOLO_EINVAL (nothing launched).                 */
 int holo_attention_packed(float *out, const float *q, const float *k, const float *v, int ldo, int ldq, int ldk,
                           int ldv, int head_dim, int n_heads, int n_kv_heads, const holo_batch_t *b);
 
@@ -93,8 +96,8 @@ int holo_attention_packed(float *out, const float *q, const float *k, const floa
  * one of two), rounded to bfloat16, at most 2720 in magnitude and held in f16;
  * a value is d * c, c the nearest to x / d in -8 .. 7 (ties to the even one).
  * d has 8 significant bits, so d * c is an f16 and the products below are of
- * exact operands.  A block that holds an infinity or NaN reads as NaN; values
- * past 21760 are held as about that.
+ * exact operands (holo_kv4_append writes no other scales).  A block that holds an
+ * infinity or NaN reads as NaN; values past 21760 are held as about that.
  *
  * pool, table and len are device memory of the caller.  Entry p of a sequence's
  * row of `table` is the page of its positions p * page_len ..; an entry outside
@@ -117,7 +120,8 @@ typedef struct {
 size_t holo_kv4_page_bytes(const holo_kv4_t *c);
 /* The batch's rows of k and v ([n_kv_heads * head_dim] floats, ldk and ldv from
  * one row to the next) into the pages of one layer, at the last positions of
- * their sequences.  What the other positions hold stays.  0 or HOLO_EINVAL.     */
+ * their sequences, shared pages among them (reserve first).  What the other
+ * positions hold stays.  0 or HOLO_EINVAL.                                      */
 int holo_kv4_append(const holo_kv4_t *c, int layer, const float *k, const float *v, int ldk, int ldv,
                     const holo_batch_t *b);
 /* The values that the cache holds for the batch's rows (zeros where there is no page). */
@@ -127,8 +131,10 @@ int holo_kv4_read(const holo_kv4_t *c, int layer, float *k, float *v, int ldk, i
  * (cuda_multi_head_attention over several sequences, cuda_ops.h:112; with more
  * rows holo_attention_prefill).  A row that sees no position gives zeros; the
  * rows of a sequence longer than max_len give NaN.  q rows of n_heads *
- * head_dim floats.  0 or HOLO_EINVAL; without memory for its partial sums the
- * hipError_t.                                                                  */
+ * head_dim floats; scores past a float's range give NaN, or zeros where every one is
+ * below it.  max_rows up to 65535, and its tiles of 16 columns (a row's heads
+ * of one KV head) times n_kv_heads too.  0 or HOLO_EINVAL; without memory for
+ * its partial sums the hipError_t.                                             */
 int holo_attention_kv4(const holo_kv4_t *c, int layer, float *out, const float *q, int ldo, int ldq, int n_heads,
                        const holo_batch_t *b);
 /* Page dst[i] becomes a copy of page src[i], every layer (host arrays).
