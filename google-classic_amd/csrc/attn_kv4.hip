@@ -99,14 +99,15 @@ __device__ __forceinline__ void load_v(TileV<NB> &t, const uint8_t *at, uint32_t
     for (int b = 0; b < NB; b++) t.s[b] = *(const u4 *)(at + 1088 * NB + 64 * b + 16 * (lane >> 4));
 }
 
+constexpr int kLeastRange = 8;  // tiles (of at least 4: 8000 positions of one sequence 12.2 us, of 8 10.1)
+
 struct Kv4Attn {
     Kv4View c;
     holo_batch_t b;
     float *out, *part;
     const float *q;
     int ldo, ldq, n_heads;
-    int chunk;   // tiles of a range
-    int splits;  // ranges a sequence of max_len positions has
+    int splits;  // the most ranges that a sequence is cut into
     int ctiles;  // tiles of 16 columns that max_rows rows have
 };
 
@@ -115,6 +116,12 @@ struct Kv4Attn {
 __device__ __forceinline__ float *partial(const Kv4Attn &a, int entry, int row, int h, int hd)
 {
     return a.part + ((((int64_t)entry * a.b.max_rows + row) * a.n_heads + h) * a.splits) * (hd + 4);
+}
+
+// Tiles of a range of a sequence that has n.
+__device__ __forceinline__ int range_of(const Kv4Attn &a, int n)
+{
+    return a.splits == 1 ? max(n, 1) : max((n + a.splits - 1) / a.splits, kLeastRange);
 }
 
 // Column c of an entry and KV head: row c / G, query head kvh * G + c % G.
@@ -137,7 +144,7 @@ __global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
     const int from = e.len - e.rows;
     const int see = max(from + last_row + 1, 0);  // positions the last row sees
     const int ntiles = too_long ? 0 : (see + 31) >> 5;
-    const int t0 = blockIdx.x * a.chunk, t1 = min(t0 + a.chunk, ntiles);
+    const int chunk = range_of(a, ntiles), t0 = blockIdx.x * chunk, t1 = min(t0 + chunk, ntiles);
     if (t0 >= ntiles && blockIdx.x > 0) return;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -329,7 +336,7 @@ __global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
     }
     __syncthreads();
     // one range: the entry's tiles are all here
-    const bool whole = a.splits == 1 || ntiles <= a.chunk;
+    const bool whole = ntiles <= chunk;
     for (int i = threadIdx.x; i < 16 * (HD / 4); i += 64 * W) {
         const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
         if (c0 + c >= ncols) continue;
@@ -375,7 +382,7 @@ __global__ __launch_bounds__(256) void attn_kv4_join_k(Kv4Attn a)
     // the ranges of the row's tile of columns, as the workgroups above have it
     const int c0 = (row * G + h % G) & ~15, last_row = (min(c0 + 16, e.take * G) - 1) / G;
     const int ntiles = (max(e.len - e.rows + last_row + 1, 0) + 31) >> 5;
-    const int n = (ntiles + a.chunk - 1) / a.chunk;
+    const int chunk = range_of(a, ntiles), n = (ntiles + chunk - 1) / chunk;
     if (n <= 1) return;
     const int64_t at = e.first + row;
     const float *pp = partial(a, blockIdx.z, row, h, HD);
@@ -427,18 +434,16 @@ __global__ __launch_bounds__(256) void attn_kv4_join_k(Kv4Attn a)
     *(f4 *)(a.out + at * a.ldo + (int64_t)h * HD + d) = O * (L == 0.f ? 0.f : 1.0f / L);
 }
 
-// Tiles of a range: all of a sequence where it has few (700 positions of 32
-// sequences, a workgroup a CU: 9.7 us, in two ranges 13.4, the launch that joins
-// them among it; 513 of one: 8.5, in three 8.9) or where there are two workgroups
-// a CU without ranges (64 sequences of up to 8192: 104, in ranges of 4096
-// positions 118); else as many ranges as bring it there, of at least 8 tiles (one
-// of 8000: 10.1, of at least 4 12.2).
-static int range_tiles(int64_t groups, int tiles)
+// Ranges: one where a sequence has few tiles (700 positions of 32 sequences, a
+// workgroup a CU: 9.7 us, in two ranges 13.4, the launch that joins them among it;
+// 513 of one: 8.5, in three 8.9) or where there are two workgroups a CU without
+// ranges (64 sequences of up to 8192: 104, in two 118); else as many as bring it
+// there.  max_len only bounds them: each sequence's own tiles are dealt out evenly.
+static int ranges(int64_t groups, int tiles)
 {
-    if (tiles <= 24) return 24;
-    const int64_t want = (2 * (int64_t)num_cus() + groups - 1) / groups;
-    const int64_t chunk = (tiles + want - 1) / want;
-    return (int)(chunk < 8 ? 8 : chunk);
+    if (tiles <= 24) return 1;
+    const int64_t want = (2 * (int64_t)num_cus() + groups - 1) / groups, most = (tiles + kLeastRange - 1) / kLeastRange;
+    return (int)(want < most ? want : most);
 }
 
 template <int NB>
@@ -449,8 +454,7 @@ static int run_attn(Kv4Attn a)
     a.ctiles = (int)(((int64_t)take * G + 15) / 16);
     const int tiles = (a.b.max_len + 31) / 32;
     const int64_t groups = (int64_t)a.ctiles * a.c.n_kv_heads * a.b.n_seqs;
-    a.chunk = range_tiles(groups, tiles);
-    a.splits = max(1, (tiles + a.chunk - 1) / a.chunk);
+    a.splits = ranges(groups, tiles);
     const dim3 grid(a.splits, a.ctiles * a.c.n_kv_heads, a.b.n_seqs);
     constexpr size_t lds = (size_t)W * 16 * (32 * NB + 4 + 2) * sizeof(float);
     if (a.splits == 1) {
@@ -485,7 +489,7 @@ extern "C" int holo_attention_kv4(const holo_kv4_t *c, int layer, float *out, co
     }
     if (b->rows == 0 || b->n_seqs == 0) return 0;
     const int64_t dim = (int64_t)n_heads * c->head_dim;
-    Kv4Attn a{kv4_view(c, layer), *b, out, nullptr, q, ldo, ldq, n_heads, 0, 0, 0};
+    Kv4Attn a{kv4_view(c, layer), *b, out, nullptr, q, ldo, ldq, n_heads, 0, 0};
     a.b.max_rows = b->max_rows < b->rows ? b->max_rows : b->rows;
     const int64_t cols = (int64_t)a.b.max_rows * (n_heads / c->n_kv_heads);
     if (!rows_ok(q, ldq, dim) || !rows_ok(out, ldo, dim) || b->max_len < 0 || b->max_len > 0x7FFFF000 ||
