@@ -27,8 +27,8 @@
 // them unpacking) issue in 56% of the cycles, 72% of those in which a CU has work,
 // the rest is the lengths' imbalance.  One wave's tile is a chain of 1.2 us: 513
 // positions of one sequence (four tiles a wave) 8.5 us, 16 sequences of up to 4096
-// (eight) 19 and 4.8 for the ranges' join, which for 100000 positions of one
-// sequence is 4.9 of 32.  Chunks: 16 columns unpack every tile again, four
+// (up to eight) 15.2 and 4.8 for the ranges' join, which for 100000 positions of
+// one sequence is 4.9 of 32.  Chunks: 16 columns unpack every tile again, four
 // sequences of 100 rows at 2000 take 37-40 us at 270 TFLOP/s.  With the tiles in LDS
 // for 128 columns that was 62, with 32 columns a wave as fast or slower (the second
 // operand's registers), with q in LDS or eight waves 5-15% slower.

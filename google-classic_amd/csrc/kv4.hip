@@ -296,7 +296,8 @@ static void copy_pages(const holo_kv4_t *c, const int *src, const int *dst, int 
 
 bool kv4_layout_ok(const holo_kv4_t *c)
 {
-    if (!c || c->n_pages <= 0 || c->n_layers <= 0 || c->n_kv_heads <= 0 || c->n_kv_heads > 65535) return false;
+    if (!c || c->n_pages <= 0 || c->n_layers <= 0 || c->n_layers > 65535 || c->n_kv_heads <= 0 || c->n_kv_heads > 65535)
+        return false;
     const int p = c->page_len, h = c->head_dim;
     return p >= 32 && p <= 1024 && !(p & (p - 1)) && (h == 32 || h == 64 || h == 96 || h == 128);
 }

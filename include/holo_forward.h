@@ -111,7 +111,7 @@ typedef struct {
     const int *len;   /* [n_seqs] */
     int n_pages;
     int page_len;     /* 32, 64, 128, 256, 512 or 1024 */
-    int n_layers, n_kv_heads;
+    int n_layers, n_kv_heads; /* up to 65535 */
     int head_dim;     /* 32, 64, 96 or 128 */
     int n_seqs, max_pages;
 } holo_kv4_t;

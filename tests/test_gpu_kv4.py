@@ -212,7 +212,7 @@ def test_attention_of_a_long_sequence_is_joined_from_ranges(holo):
     q = (3 * rng.standard_normal((3, heads * hd))).astype(np.float32)
     want = want_attention(c, 0, q, [1, 1, 1], c.len, [0, 1, 2], heads)
     first = attention(holo, dev, 0, q, [1, 1, 1], heads)
-    for got in (first, attention(holo, dev, 0, q, [1, 1, 1], heads, max_len=2560 * 8 // 8),
+    for got in (first, attention(holo, dev, 0, q, [1, 1, 1], heads, max_len=2560),
                 attention(holo, dev, 0, q, [1, 1, 1], heads, max_len=100000)):
         assert normwise(got, want) <= TOL
     assert np.array_equal(first, attention(holo, dev, 0, q, [1, 1, 1], heads))
@@ -512,3 +512,76 @@ def test_scores_far_past_the_exponential(holo, scale):
         assert first - second > 1e-4 * first
         # p is 2^7.5 in two halves, and its sum the same number
         assert np.abs(got[h] - v[s.argmax()]).max() <= 2.0 ** -21 * np.abs(v[s.argmax()]).max()
+
+
+@pytest.mark.parametrize("lens", [[1, 40, 255, 256, 257, 600], [3000, 2, 800]], ids=str)
+def test_ranges_follow_the_lengths(holo, lens):
+    """A bound on the lengths far above them: the sequences' own tiles are dealt out, one to many ranges."""
+    print(f"case kv4 ranges {lens}", flush=True)
+    rng = np.random.default_rng(14)
+    hd, heads, n_kv = 32, 4, 1
+    c = Cache(hd, 128, 1, n_kv, sum(-(-n // 128) for n in lens), len(lens), 24)
+    pages(c, lens, rng)
+    fill(c, rng, lens, 0)
+    dev = OnDevice(holo, c)
+    rows = [min(n, 5) for n in lens]
+    q = rng.standard_normal((sum(rows), heads * hd)).astype(np.float32)
+    want = want_attention(c, 0, q, rows, c.len, list(range(len(lens))), heads)
+    for bound in (c.len.max(), 3200, 40000, 1 << 20, 0x7FFFF000):
+        if bound >= c.len.max():
+            assert normwise(attention(holo, dev, 0, q, rows, heads, max_len=bound), want) <= TOL
+
+
+def test_pages_on_the_device_follow_the_bookkeeping(holo):
+    """More updates and copies than one launch takes: a long sequence, its fork, the pages compacted."""
+    print("case kv4 bookkeeping", flush=True)
+    rng = np.random.default_rng(15)
+    lib = holo.lib()
+    c = Cache(32, 32, 1, 1, 1500, 4, 700)
+    dev = OnDevice(holo, c)
+    p = lib.holo_kv4_pages_create(dev.ref)
+    assert p
+    ints = lambda *x: np.int32(x)
+
+    def call(name, *arrays):
+        assert getattr(lib, name)(p, *[a.ctypes.data for a in arrays], len(arrays[0])) == 0
+
+    def device():
+        lib.cuda_sync()
+        holo.check("bookkeeping")
+        return dev.table.download(np.int32).reshape(4, 700), dev.len.download(np.int32)
+
+    def listed():
+        table, lens = np.full((4, 700), -1, np.int32), np.zeros(4, np.int32)
+        for s in range(4):
+            n = lib.holo_kv4_pages_list(p, s, table[s].ctypes.data, 700)
+            lens[s] = lib.holo_kv4_pages_len(p, s)
+            assert n == -(-lens[s] // 32)
+        return table, lens
+
+    def same():
+        (t, n), (t2, n2) = device(), listed()
+        assert np.array_equal(t, t2) and np.array_equal(n, n2)
+        return t, n
+
+    try:
+        same()
+        call("holo_kv4_pages_reserve", ints(2, 0), ints(620 * 32, 650 * 32 - 5))
+        same()
+        call("holo_kv4_pages_fork", ints(0), ints(3))
+        t, _ = same()
+        before = dev.bytes()
+        assert np.array_equal(t[0], t[3])
+        call("holo_kv4_pages_reserve", ints(3), ints(40))  # a shared last page and new ones
+        t, n = same()
+        assert n[3] == 650 * 32 + 35 and np.array_equal(t[0, :649], t[3, :649]) and t[0, 649] != t[3, 649]
+        assert np.array_equal(dev.bytes()[t[3, 649]], before[t[0, 649]])
+        call("holo_kv4_pages_free", ints(2))
+        held = dev.bytes()[same()[0][3, :650]]
+        assert lib.holo_kv4_pages_compact(p) == 0  # more than 256 pages move
+        t, n = same()
+        used = set(t[t >= 0].tolist())
+        assert used == set(range(len(used))) and np.array_equal(dev.bytes()[t[3, :650]], held)
+        assert lib.holo_kv4_pages_available(p) == 1500 - len(used)
+    finally:
+        lib.holo_kv4_pages_destroy(p)

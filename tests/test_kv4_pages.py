@@ -35,6 +35,17 @@ def test_page_bytes():
     assert lib.holo_kv4_page_bytes(None) == 0
 
 
+def test_sizes_past_the_limits_are_refused():
+    lib = h.lib()
+    assert lib.holo_kv4_page_bytes(C.byref(layout(n_layers=65535))) > 0
+    assert lib.holo_kv4_page_bytes(C.byref(layout(n_layers=65536))) == 0
+    c = layout(**POINTERS)
+    b = h.Batch(rows=0x7FFFF001, n_seqs=2, max_rows=1, max_len=64, cu_rows=16384)
+    assert rejected(lib.holo_kv4_append(C.byref(c), 0, 4096, 8192, 128, 128, C.byref(b)))
+    assert rejected(lib.holo_attention_kv4(C.byref(c), 0, 4096, 8192, 256, 256, 4, C.byref(b)))
+    assert rejected(lib.holo_attention_packed(4096, 8192, 4096, 8192, 256, 256, 128, 128, 64, 4, 2, C.byref(b)))
+
+
 POINTERS = dict(pool=4096, table=8192, len=12288)
 
 
