@@ -16,7 +16,7 @@
 //     they stand.  Pieces are permuted (XOR) so that the writes and the reads of 16
 //     lanes fall on 64 different banks.
 //   - Keys and values are held times 2^8, which suits f16 for rows whose largest
-//     value is in [2^-11, 2^8); q rows are scaled to their largest value.  Smaller
+//     value is in [2^-11, 255.9375); q rows are scaled to their largest value.  Smaller
 //     rows are held within 2^-33, which does no harm to scores of ordinary q rows, nor
 //     to outputs that other rows have a part in.  The columns that it harms, and
 //     every column of a workgroup that walks a row of larger values (or of infinities
@@ -48,8 +48,9 @@ struct PackedAttn {
     int ldo, ldq, ldk, ldv, n_heads, n_kv_heads;
 };
 
-constexpr float kHeld = 256.f;                               // keys and values are held times this
-constexpr float kRowLow = 1.f / 2048.f, kRowHigh = 256.f;    // a row's largest value
+constexpr float kHeld = 256.f;  // keys and values are held times this
+// A row's largest value; from kRowHigh up, times kHeld it is 65520 and more, which f16 rounds to infinity.
+constexpr float kRowLow = 1.f / 2048.f, kRowHigh = 255.9375f;
 // What a workgroup's staged rows hold that the halves do not suit.  Low rows are
 // held within 2^-33: no harm to a column whose scores that moves by 2^-22 at most (hd
 // values of q below 16 in log2 units, sc below kLowSc), or whose output's

@@ -1,0 +1,46 @@
+"""holo_attention_packed at the magnitudes where its forms change, against
+float64 numpy, in every form of the kernel.
+
+Tolerance 1e-5 normwise, as for values of ordinary size: the planted products are
+kept at an ordinary score's size (q is small where a key is large), and a
+planted value's part is its probability, within 2e-6 in the mean, times it."""
+import numpy as np
+import pytest
+
+from test_gpu_packed_attention import TOL, inputs, normwise, run
+
+pytestmark = pytest.mark.gpu
+
+# head_dim, heads, KV heads, rows: keys shared by eight waves, by four, 128 columns (two), 256 columns
+FORMS = [(128, 4, 2, [100]), (128, 32, 32, [300]), (128, 8, 4, [30, 12]), (64, 64, 64, [600]), (96, 64, 64, [1030])]
+
+
+def want_head(q, k, v, n, hd, h, g):
+    """Rows 0 .. n - 1 of one sequence and head, in 64 bits."""
+    kh, vh = (x[:n, g * hd:(g + 1) * hd].astype(np.float64) for x in (k, v))
+    with np.errstate(invalid="ignore"):
+        s = q[:n, h * hd:(h + 1) * hd].astype(np.float64) @ kh.T / np.sqrt(hd)
+        s[np.arange(n)[None] > np.arange(n)[:, None]] = -np.inf
+        p = np.exp(s - s.max(1, keepdims=True))
+        return (p / p.sum(1, keepdims=True)) @ vh
+
+
+@pytest.mark.parametrize("hd,heads,n_kv,rows", FORMS, ids=str)
+@pytest.mark.parametrize("value", [False, True], ids=["key", "value"])
+def test_around_the_largest_value_of_the_halves(holo, hd, heads, n_kv, rows, value):
+    """Times 2^8, f16 rounds values from 255.9375 up to infinity: the rows that see a key or
+    value just below, at and past that, and the rows before it."""
+    total, n = sum(rows), rows[0]
+    at, dim = n // 2, 5
+    for x in (255.9374, 255.9375, -255.9375, -255.99, 256.0):
+        print(f"case packed hd {hd} heads {heads}/{n_kv} rows {rows} {'value' if value else 'key'} {x}", flush=True)
+        q, k, v = inputs(31, total, hd, heads, n_kv)
+        q[:, dim::hd] /= 64
+        (v if value else k)[at, dim::hd] = x
+        got = run(holo, q, k, v, rows, hd, heads, n_kv)
+        assert np.isfinite(got).all()
+        for h in (0, heads - 1):
+            want = want_head(q, k, v, n, hd, h, h * n_kv // heads)
+            part = got[:n, h * hd:(h + 1) * hd]
+            assert normwise(part[:at], want[:at]) <= TOL
+            assert normwise(part[at:], want[at:]) <= TOL
