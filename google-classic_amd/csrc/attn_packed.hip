@@ -141,9 +141,10 @@ __device__ __forceinline__ void packed_fp32(const PackedAttn &a, const float *qp
         l = was;
 #pragma unroll
         for (int n = 0; n < N; n++) l += s[n] = __builtin_amdgcn_exp2f(s[n] - mx);
-        const float keep = was / l;
+        // (while every score is -infinity no key has weight, and the average stays 0)
+        const float sum = l == 0.f ? 1.f : l, keep = was / sum;
 #pragma unroll
-        for (int n = 0; n < N; n++) s[n] /= l;
+        for (int n = 0; n < N; n++) s[n] /= sum;
 #pragma unroll
         for (int i = 0; i < H / 4; i++) {
             f4 y = o[i] * keep;
@@ -159,7 +160,7 @@ __device__ __forceinline__ void packed_fp32(const PackedAttn &a, const float *qp
     for (; key + 3 <= row; key += 4) keys.template operator()<4>(key);
     for (; key <= row; key++) keys.template operator()<1>(key);
 #pragma unroll
-    for (int i = 0; i < H / 4; i++) ((f4 *)out)[i] = o[i];
+    for (int i = 0; i < H / 4; i++) ((f4 *)out)[i] = l == 0.f ? f4{NAN, NAN, NAN, NAN} : o[i];
 }
 
 // W = 4: 128 columns a workgroup, each wave doing all of a tile's work, the next

@@ -81,9 +81,11 @@ typedef struct {
  * every ld a multiple of 4, ldk and ldv below 2^24; max_rows times n_heads /
  * n_kv_heads up to 2097120.  seqs and max_len are not read.  A row is not
  * touched by what the rows behind it hold, infinities and NaN among it.  Any
- * magnitude is right; keys or values of 255.9375 and more (and rows of which
- * none reaches 2^-11, where they make up an output) take an fp32 path some
- * thirty times slower.  Returns 0 or HOLO_EINVAL (nothing launched).           */
+ * magnitude is right whose scores are floats: a key whose score lies below a
+ * float's range has no part, one above it or no key with a part makes the row
+ * and head NaN.  Keys or values of 255.9375 and more (and rows of which none
+ * reaches 2^-11, where they make up an output) take an fp32 path some thirty
+ * times slower.  Returns 0 or HOLO_EINVAL (nothing launched).                  */
 int holo_attention_packed(float *out, const float *q, const float *k, const float *v, int ldo, int ldq, int ldk,
                           int ldv, int head_dim, int n_heads, int n_kv_heads, const holo_batch_t *b);
 

@@ -44,3 +44,26 @@ def test_around_the_largest_value_of_the_halves(holo, hd, heads, n_kv, rows, val
             part = got[:n, h * hd:(h + 1) * hd]
             assert normwise(part[:at], want[:at]) <= TOL
             assert normwise(part[at:], want[at:]) <= TOL
+
+
+@pytest.mark.parametrize("hd,heads,n_kv,rows", FORMS, ids=str)
+@pytest.mark.parametrize("low", [-np.inf, -3e38], ids=["infinite", "finite"])
+def test_first_keys_without_weight(holo, hd, heads, n_kv, rows, low):
+    """Scores of -infinity (or of less than a float holds) at a sequence's first keys, one to
+    five of them, and at one in its middle: those keys have no part in the rows that see others,
+    and rows that see no others are NaN, as the formula's difference of two infinities."""
+    total, n, dim = sum(rows), rows[0], 3
+    for first in (1, 2, 4, 5):
+        print(f"case packed hd {hd} heads {heads}/{n_kv} rows {rows} first {first} keys of {low}", flush=True)
+        q, k, v = inputs(32, total, hd, heads, n_kv)
+        q[:, dim::hd] = 4 + np.abs(q[:, dim::hd])
+        # other keys: a dim's products of an ordinary score's size
+        k[:, dim::hd] /= 8
+        for at in (*range(first), n // 2):
+            k[at, dim::hd] = low
+        got = run(holo, q, k, v, rows, hd, heads, n_kv)
+        for h in (0, heads - 1):
+            want = want_head(q, k, v, n, hd, h, h * n_kv // heads)
+            part = got[:n, h * hd:(h + 1) * hd]
+            assert np.isnan(part[:first]).all()
+            assert normwise(part[first:], want[first:]) <= TOL
