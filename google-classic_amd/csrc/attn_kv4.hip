@@ -23,13 +23,14 @@
 // launch joins in range order.
 //
 // What bounds it (32 heads on 8 of 128): 64 sequences of up to 8192 positions, 455
-// MB, take 100-114 us, 4.0-4.6 TB/s; vector instructions (300 a tile, 192 of
+// MB, take 100-116 us, 3.9-4.6 TB/s; vector instructions (300 a tile, 192 of
 // them unpacking) issue in 56% of the cycles, 72% of those in which a CU has work,
 // the rest is the lengths' imbalance.  One wave's tile is a chain of 1.2 us: 513
-// positions of one sequence (four tiles a wave) 8.5 us, 16 sequences of up to 4096
-// (up to eight) 15.2 and 4.8 for the ranges' join, which for 100000 positions of
-// one sequence is 4.9 of 32.  Chunks: 16 columns unpack every tile again, four
-// sequences of 100 rows at 2000 take 37-40 us at 270 TFLOP/s.  With the tiles in LDS
+// positions of one sequence (four tiles a wave) 8.5 us.  16 sequences of up to 4096
+// (up to eight) 17.8: 15.3 and 4.8 for the ranges' join in a kernel trace, whose
+// times hold each launch's start and end.  100000 positions of one sequence 32-34,
+// the join 5.1 of them.  Chunks: 16 columns unpack every tile again, four
+// sequences of 100 rows at 2000 take 37-40 us at 260 TFLOP/s.  With the tiles in LDS
 // for 128 columns that was 62, with 32 columns a wave as fast or slower (the second
 // operand's registers), with q in LDS or eight waves 5-15% slower.
 #include "attn_tiles.h"
@@ -439,6 +440,9 @@ __global__ __launch_bounds__(256) void attn_kv4_join_k(Kv4Attn a)
 // 513 of one: 8.5, in three 8.9) or where there are two workgroups a CU without
 // ranges (64 sequences of up to 8192: 104, in two 118); else as many as bring it
 // there.  max_len only bounds them: each sequence's own tiles are dealt out evenly.
+// (Every entry counts with max_rows rows.  Beside a chunk of 512 rows at 2000, 70 us by
+// itself, one token at 100000 walks its sequence in one range: 999 us, alone 31; with
+// 15 tokens at up to 4096, alone 23.6, the chunk takes 268.)
 static int ranges(int64_t groups, int tiles)
 {
     if (tiles <= 24) return 1;
@@ -462,7 +466,9 @@ static int run_attn(Kv4Attn a)
         HOLO_LAUNCH_CHECK();
         return 0;
     }
-    // (a small buffer: ranges are for fewer than two workgroups a CU, and make fewer than four)
+    // (a small buffer: ranges are for fewer than two workgroups a CU, and make fewer than
+    // four.  At two, with 4 heads a KV head of 128 dims, it is 1.03 MiB, which a captured call
+    // allocates by nodes of its graph: 16 sequences of up to 4096 20.1 us eager, 29-31 replayed.)
     const StreamScratch scratch((size_t)a.b.n_seqs * take * a.n_heads * a.splits * (32 * NB + 4) * sizeof(float));
     a.part = (float *)scratch.get();
     if (!a.part) {

@@ -28,10 +28,10 @@
 // KV heads are the fastest grid index, so that with 8 of them each XCD's L2 holds
 // one head's keys and values.
 //
-// What bounds it: 4096 rows, 32 heads on 8 of 128, take 365 us, three products of
-// 137 GFLOP each at 1.13 PFLOP/s; a large f16 product of the library runs at 1.22 on
-// such values, the chip's power setting both (the matrix cores are busy 64% of the
-// cycles, at 1.7 GHz).  Below that, the steps that led here: 16 columns a workgroup
+// What bounds it: 4096 rows, 32 heads on 8 of 128, take 357 us (355-425 on several
+// cards), three products of 137 GFLOP each at 1.15 PFLOP/s; a large f16 product of the
+// library runs at 1.22 on such values, the chip's power setting both (the matrix cores
+// are busy 64% of the cycles, at 1.7 GHz).  Below that, the steps that led here: 16 columns a workgroup
 // and every tile split by each 2703 us, 128 columns 622, nothing spilled 463,
 // cheaper halves and checks 437.  Short prompts: one chain of loads, scores,
 // exponentials and products a tile, 7.4 us with one tile.
@@ -814,9 +814,12 @@ static void launch_packed(const PackedAttn &a, int64_t cols)
 //   of 64 rows 26.0, 35.1 14.3 19.2), where there is nothing to share;
 //   128 columns, with 32 keys at most (one row 7.4; 8.9 8.5 9.2) and from there on;
 //   256 in two groups where they fill the chip with long prompts: 4096 rows 365-391
-//   (436-464 with 128), four of up to 1023 77.8 (81.1); 16 of 256 rows 61.9
-//   (59.9), and with head_dim 64, where more waves of 128 fit a SIMD, four of 1024
-//   92.6 (81.1).
+//   (436-464 with 128), two of 1000 72.7 (90.4), four 128.5 (129.9), 16 of 999 475
+//   (496); 16 of 256 rows 61.9 (59.9), eight of 384 63.2 (59.6), and with head_dim 64,
+//   where more waves of 128 fit a SIMD, four of 1024 92.6 (81.1).  Between 500 and
+//   1000 rows, which take 128 columns, the two are level (four of 640 65.7, 64.4;
+//   head_dim 96, eight of 768 134.8, 132.3) or 256 are faster (four of 512 46.5,
+//   54.0; four of 768 86.3, 95.2; two of 999 73.0, 90.7).
 template <int NB>
 static void run_packed(const PackedAttn &a, int64_t cols)
 {

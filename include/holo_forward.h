@@ -85,7 +85,8 @@ typedef struct {
  * float's range has no part, one above it or no key with a part makes the row
  * and head NaN.  Keys or values of 255.9375 and more (and rows of which none
  * reaches 2^-11, where they make up an output) take an fp32 path some thirty
- * times slower.  Returns 0 or HOLO_EINVAL (nothing launched).                  */
+ * times slower; others are held within 2^-22 of themselves, or within 2^-33
+ * where that is more.  Returns 0 or HOLO_EINVAL (nothing launched).            */
 int holo_attention_packed(float *out, const float *q, const float *k, const float *v, int ldo, int ldq, int ldk,
                           int ldv, int head_dim, int n_heads, int n_kv_heads, const holo_batch_t *b);
 
@@ -135,8 +136,10 @@ int holo_kv4_read(const holo_kv4_t *c, int layer, float *k, float *v, int ldk, i
  * rows of a sequence longer than max_len give NaN.  q rows of n_heads *
  * head_dim floats; scores past a float's range give NaN, or zeros where every one is
  * below it.  max_rows up to 65535, and its tiles of 16 columns (a row's heads
- * of one KV head) times n_kv_heads too.  0 or HOLO_EINVAL; without memory for
- * its partial sums the hipError_t.                                             */
+ * of one KV head) times n_kv_heads too.  Long sequences are cut into ranges, as
+ * many as entries of max_rows rows each leave room for: single tokens are faster
+ * in a call of their own than beside a chunk of many rows.  0 or HOLO_EINVAL;
+ * without memory for its partial sums the hipError_t.                          */
 int holo_attention_kv4(const holo_kv4_t *c, int layer, float *out, const float *q, int ldo, int ldq, int n_heads,
                        const holo_batch_t *b);
 /* Page dst[i] becomes a copy of page src[i], every layer (host arrays).
