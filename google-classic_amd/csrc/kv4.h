@@ -69,6 +69,7 @@ __device__ __forceinline__ int word_shift(int i) { return 4 * (i >> 1) + 16 * (i
 bool kv4_layout_ok(const holo_kv4_t *c);
 bool kv4_call_ok(const holo_kv4_t *c, int layer, const holo_batch_t *b);
 bool batch_ok(const holo_batch_t *b);
+bool draft_rows_ok(const holo_batch_t *b, int words);  // an entry's rows have a bit each in so many words
 Kv4View kv4_view(const holo_kv4_t *c, int layer);
 // Rows at p, ld floats from one to the next, of `dim` floats, in 16-byte pieces.
 inline bool rows_ok(const void *p, int ld, int64_t dim) { return p && !((uintptr_t)p & 15) && ld % 4 == 0 && ld >= dim; }

@@ -1,8 +1,6 @@
 // kv4.hip -- the 4-bit cache (holo_forward.h): rows in and out of its pages,
 // page copies, and the host bookkeeping of which page is whose.
-#include "kv4.h"
-
-#include <float.h>
+#include "kv4_quant.h"
 
 #include <algorithm>
 #include <functional>
@@ -13,70 +11,6 @@
 #include <vector>
 
 namespace holo {
-
-// ---- quantisation of a block of 32 ----------------------------------------------------
-//
-// Eight lanes hold a block, four values each.  The code is the nearest integer
-// to x / d.  x * (1 / d) is within 2^-20 of it, so its nearest integer is the code
-// unless it lies that near to the middle of two; there the remainder x - c d
-// decides (exact: c d has 12 bits and x lies within a factor of c d).
-
-// The larger (or smaller) of the eight lanes' values; NaN if one is.
-template <bool MAX>
-__device__ __forceinline__ float of_eight(float v)
-{
-    auto pick = [](float a, float b) { return MAX ? __builtin_elementwise_maximum(a, b) : __builtin_elementwise_minimum(a, b); };
-    v = pick(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false)));   // quad [1,0,3,2]
-    v = pick(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false)));   // quad [2,3,0,1]
-    return pick(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false)));  // half mirror
-}
-
-// f16 bits of the block's scale: bfloat16(|m| / 8), at most 2720, and m's sign
-// reversed; NaN where a value is not finite.
-__device__ __forceinline__ uint16_t kv4_scale(const float4 x)
-{
-    auto least = [](float a, float b) { return __builtin_elementwise_minimum(a, b); };
-    auto most = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };
-    const float lo = of_eight<false>(least(least(x.x, x.y), least(x.z, x.w)));
-    const float hi = of_eight<true>(most(most(x.x, x.y), most(x.z, x.w)));
-    const float big = most(-lo, hi);
-    const uint32_t u = __float_as_uint(big * 0.125f);
-    const float b = __uint_as_float((u + 0x7FFFu + ((u >> 16) & 1u)) & 0xFFFF0000u);  // bfloat16, ties to even
-    const float d = fminf(b, 2720.f);
-    const uint16_t h = __builtin_bit_cast(uint16_t, (_Float16)(-lo >= hi ? d : -d));
-    return big <= FLT_MAX ? h : (uint16_t)0x7E00;
-}
-
-// The lane's four codes, one a byte.
-__device__ __forceinline__ uint32_t kv4_codes(const float4 x4, uint16_t scale)
-{
-    const float d = (float)__builtin_bit_cast(_Float16, scale);
-    if (!(fabsf(d) > 0.f)) return 0x08080808u;  // zeros, and blocks of NaN
-    const float inv = 1.0f / d, x[4] = {x4.x, x4.y, x4.z, x4.w};
-    float c[4];
-    bool near = false;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float q = fminf(fmaxf(x[i] * inv, -9.f), 9.f);
-        c[i] = rintf(q);
-        near |= fabsf(q - c[i]) > 0.5f - 0x1p-16f;
-    }
-    if (near) {
-        const float h = 0.5f * fabsf(d);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float r = fmaf(-c[i], d, x[i]);
-            r = d < 0.f ? -r : r;
-            const bool odd = (int)c[i] & 1;
-            if (r > h || (r == h && odd)) c[i] += 1.f;
-            else if (r < -h || (r == -h && odd)) c[i] -= 1.f;
-        }
-    }
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) w |= (uint32_t)((int)fminf(fmaxf(c[i], -8.f), 7.f) + 8) << (8 * i);
-    return w;
-}
 
 // Words of V in a tile, and the place of word (m, lane g, r) among them.
 template <int NB>
@@ -115,8 +49,8 @@ template <int NB>
 __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, const float *k, const float *v, int ldk,
                                                     int ldv)
 {
-    constexpr int HD = 32 * NB, VW = VWords<NB>::W, M = 2 * NB;
-    __shared__ __align__(16) uint8_t lv[32][HD];  // [position][16 r's][M dims r + 16 m]
+    constexpr int HD = 32 * NB;
+    __shared__ __align__(16) uint8_t lv[32 * HD];
     const Kv4Entry e = kv4_entry(c, b, blockIdx.z);
     const int kvh = blockIdx.y, from = e.len - e.rows;  // position of the entry's first row
     if ((int)blockIdx.x > (e.take + 30) / 32) return;  // (so that 32 t stays an int)
@@ -126,59 +60,17 @@ __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, c
     if (lo >= hi) return;
     uint8_t *tile = kv4_tile<NB>(c, e, kvh, t);
     if (!tile) return;
-    uint32_t *kw = (uint32_t *)tile, *vw = (uint32_t *)(tile + 16 * HD);
-    uint16_t *ks = (uint16_t *)(tile + 32 * HD), *vs = (uint16_t *)(tile + 34 * HD);
-    // the thread's words of V, VW of lane group vg, and which of their nibbles are new
-    const int vg = threadIdx.x >> 4 & 3, vr = threadIdx.x & 15, vc = threadIdx.x >> 6;
-    uint32_t mask = 0, old[VW] = {};
-    if (VW * vc < M) {
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (v_pos(vg, j) >= lo && v_pos(vg, j) < hi) mask |= 15u << word_shift(j);
-        if (mask != 0 && mask != 0xFFFFFFFFu)
-#pragma unroll
-            for (int i = 0; i < VW; i++) old[i] = vw[VW * threadIdx.x + i];
-    }
+    Kv4VWords<NB> words(tile, lo, hi);
     const int x = threadIdx.x & 7;  // the lane's place in its block
     const int64_t row0 = (int64_t)e.first + p0 - from;
     for (int i = threadIdx.x >> 3; i < (hi - lo) * NB; i += 32) {
         const int p = lo + i / NB, blk = i % NB;
         const float4 kx = *(const float4 *)(k + (row0 + p) * ldk + kvh * HD + 32 * blk + 4 * x);
         const float4 vx = *(const float4 *)(v + (row0 + p) * ldv + kvh * HD + 32 * blk + 4 * x);
-        const uint16_t kd = kv4_scale(kx), vd = kv4_scale(vx);
-        const uint32_t kc = kv4_codes(kx, kd), vcodes = kv4_codes(vx, vd);
-        // codes of values 0..3 (even lane) or 4..7 (odd): nibbles 0, 4, 1, 5 or 2, 6, 3, 7
-        uint32_t w = (kc & 15u) | (kc >> 8 & 15u) << 16 | (kc >> 16 & 15u) << 4 | (kc >> 24) << 20;
-        w <<= 8 * (x & 1);
-        w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xB1, 0xF, 0xF, false);
-        const int word = 4 * blk + (x >> 1), g = word / NB;
-        if (!(x & 1)) kw[(((p >> 4) * 4 + g) * 16 + (p & 15)) * NB + word - g * NB] = w;
-        uint8_t *to = &lv[p][4 * (x & 3) * M + 2 * blk + (x >> 2)];
-#pragma unroll
-        for (int y = 0; y < 4; y++) to[y * M] = (uint8_t)(vcodes >> (8 * y));
-        if (x == 0) {
-            ks[32 * blk + 2 * (p & 15) + (p >> 4)] = kd;
-            vs[32 * blk + 8 * ((p & 15) >> 2) + 4 * (p >> 4) + (p & 3)] = vd;
-        }
+        kv4_put<NB>(tile, lv, p, blk, x, kx, vx);
     }
     __syncthreads();
-    if (mask == 0) return;
-    uint32_t q[8];  // the codes of position j, dim i in byte i (of positions outside the batch: any four bits)
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const uint8_t *at = &lv[v_pos(vg, j)][vr * M + VW * vc];
-        q[j] = (VW == 4 ? *(const uint32_t *)at : *(const uint16_t *)at) & 0x0F0F0F0Fu;
-    }
-    // nibbles 0 and 1, 2 and 3, 4 and 5, 6 and 7 of the words: positions 0 2, 4 6, 1 3, 5 7
-    const uint32_t n0 = q[0] | q[2] << 4, n1 = q[4] | q[6] << 4, n2 = q[1] | q[3] << 4, n3 = q[5] | q[7] << 4;
-#pragma unroll
-    for (int i = 0; i < VW; i++) {
-        const uint32_t w = (n0 >> (8 * i) & 255u) | (n1 >> (8 * i) & 255u) << 8 | (n2 >> (8 * i) & 255u) << 16 |
-                           (n3 >> (8 * i) & 255u) << 24;
-        old[i] = (old[i] & ~mask) | (w & mask);
-    }
-    if constexpr (VW == 4) *(uint4 *)(vw + 4 * threadIdx.x) = make_uint4(old[0], old[1], old[2], old[3]);
-    else *(uint2 *)(vw + 2 * threadIdx.x) = make_uint2(old[0], old[1]);
+    words.store(lv);
 }
 
 // ---- read ---------------------------------------------------------------------------------
@@ -232,6 +124,100 @@ __global__ __launch_bounds__(256) void kv4_read_k(Kv4View c, holo_batch_t b, flo
         }
         *(float4 *)(k + (row0 + p) * ldk + kvh * HD + 32 * blk + 4 * x) = ko;
         *(float4 *)(v + (row0 + p) * ldv + kvh * HD + 32 * blk + 4 * x) = vo;
+    }
+}
+
+// ---- rows that stand, moved together ----------------------------------------------------------
+//
+// Row path[i] of an entry becomes its row i, in every layer and KV head: codes and
+// scales as they are.  path rises, so a row's source lies at its place or behind it;
+// a workgroup takes the tiles that it writes one after the other, reads all that
+// goes into one before it writes any of it, and no later source is among what
+// earlier tiles wrote.  A thread makes whole words: the keys of a (position, lane
+// group), the VW dims of eight positions' values.
+template <int NB>
+__global__ __launch_bounds__(NB == 3 ? 192 : 128) void kv4_keep_k(Kv4View c, holo_batch_t b, const int *path,
+                                                                 const int *n_path)
+{
+    constexpr int HD = 32 * NB, T = NB == 3 ? 192 : 128, VW = VWords<NB>::W, M = 2 * NB;
+    __shared__ const uint8_t *src[32];  // the tile that a position's row comes from; nullptr: it stays
+    __shared__ int at[32];              // and the place there
+    __shared__ int some;
+    const int s = blockIdx.z, kvh = blockIdx.x;
+    c.layer_tiles *= blockIdx.y;
+    const Kv4Entry e = kv4_entry(c, b, s);
+    const int n = min(n_path[s], e.take), from = e.len - e.rows;
+    const int end = min(from + max(n, 0), e.len);  // positions written: up to here
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    for (int t = max(from, 0) >> 5; 32 * (int64_t)t < end; t++) {
+        uint8_t *tile = kv4_tile<NB>(c, e, kvh, t);
+        if (threadIdx.x < 64) {
+            const uint8_t *of = nullptr;
+            const int i = 32 * t + (int)threadIdx.x - from;
+            if (tile && threadIdx.x < 32 && i >= 0 && i < n) {
+                const int p = path[e.first + i];
+                if (p != i && p >= 0 && p < e.rows && from + p >= 0) {
+                    of = kv4_tile<NB>(c, e, kvh, (from + p) >> 5);
+                    at[threadIdx.x] = (from + p) & 31;
+                }
+            }
+            if (threadIdx.x < 32) src[threadIdx.x] = of;
+            const bool any = __any(of != nullptr);
+            if (threadIdx.x == 0) some = any;
+        }
+        __syncthreads();
+        if (some) {
+            // keys of position 16 half + r, dims 8 (NB g ..)
+            const int half = threadIdx.x >> 6, kpos = 16 * half + r;
+            uint32_t kw[NB];
+            const uint8_t *ks = half < 2 ? src[kpos & 31] : nullptr;
+            if (ks) {
+                const uint32_t *w = (const uint32_t *)ks + NB * (64 * (at[kpos] >> 4) + 16 * g + (at[kpos] & 15));
+#pragma unroll
+                for (int j = 0; j < NB; j++) kw[j] = w[j];
+            }
+            // values of dims 16 m + r, m = VW chunk .., at eight positions
+            const int chunk = threadIdx.x >> 6;
+            uint32_t *vw = (uint32_t *)(tile + 16 * HD) + VW * threadIdx.x;
+            uint32_t old[VW], put[VW] = {}, mask = 0;
+            if (VW * chunk < M) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int p = v_pos(g, j);
+                    if (!src[p]) continue;
+                    const int sp = at[p], slot = 4 * (sp >> 4) + (sp & 3);
+                    const uint32_t *w = (const uint32_t *)(src[p] + 16 * HD) +
+                                        VW * (64 * chunk + 16 * ((sp & 15) >> 2) + r);
+                    mask |= 15u << word_shift(j);
+#pragma unroll
+                    for (int i = 0; i < VW; i++) put[i] |= (w[i] >> word_shift(slot) & 15u) << word_shift(j);
+                }
+                if (mask)
+#pragma unroll
+                    for (int i = 0; i < VW; i++) old[i] = vw[i];
+            }
+            // scales of (position, block)
+            const int sp = threadIdx.x & 31, blk = threadIdx.x >> 5;
+            uint16_t kd = 0, vd = 0;
+            const uint8_t *ss = blk < NB ? src[sp] : nullptr;
+            if (ss) {
+                const int p = at[sp];
+                kd = ((const uint16_t *)(ss + 32 * HD))[32 * blk + 2 * (p & 15) + (p >> 4)];
+                vd = ((const uint16_t *)(ss + 34 * HD))[32 * blk + 8 * ((p & 15) >> 2) + 4 * (p >> 4) + (p & 3)];
+            }
+            __syncthreads();
+            if (ks)
+#pragma unroll
+                for (int j = 0; j < NB; j++) ((uint32_t *)tile)[NB * (64 * half + lane) + j] = kw[j];
+            if (mask)
+#pragma unroll
+                for (int i = 0; i < VW; i++) vw[i] = (old[i] & ~mask) | put[i];
+            if (ss) {
+                ((uint16_t *)(tile + 32 * HD))[32 * blk + 2 * (sp & 15) + (sp >> 4)] = kd;
+                ((uint16_t *)(tile + 34 * HD))[32 * blk + 8 * ((sp & 15) >> 2) + 4 * (sp >> 4) + (sp & 3)] = vd;
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -467,6 +453,24 @@ int holo_kv4_read(const holo_kv4_t *c, int layer, float *k, float *v, int ldk, i
     return 0;
 }
 
+int holo_kv4_keep(const holo_kv4_t *c, const int *path, const int *n_path, const holo_batch_t *b)
+{
+    if (!kv4_call_ok(c, 0, b)) return rejected("holo_kv4_keep: cache or batch outside the supported set");
+    if (b->rows == 0 || b->n_seqs == 0) return 0;
+    if (!path || !n_path || ((uintptr_t)path & 3) || ((uintptr_t)n_path & 3))
+        return rejected("holo_kv4_keep: a null or misaligned array");
+    const Kv4View w = kv4_view(c, 1);  // (the kernel takes layer_tiles times its layer)
+    const dim3 grid(c->n_kv_heads, c->n_layers, b->n_seqs);
+    switch (c->head_dim) {
+    case 32: hipLaunchKernelGGL(kv4_keep_k<1>, grid, dim3(128), 0, stream(), w, *b, path, n_path); break;
+    case 64: hipLaunchKernelGGL(kv4_keep_k<2>, grid, dim3(128), 0, stream(), w, *b, path, n_path); break;
+    case 96: hipLaunchKernelGGL(kv4_keep_k<3>, grid, dim3(192), 0, stream(), w, *b, path, n_path); break;
+    default: hipLaunchKernelGGL(kv4_keep_k<4>, grid, dim3(128), 0, stream(), w, *b, path, n_path); break;
+    }
+    HOLO_LAUNCH_CHECK();
+    return 0;
+}
+
 int holo_kv4_copy_pages(const holo_kv4_t *c, const int *src, const int *dst, int n)
 {
     if (!kv4_layout_ok(c) || !c->pool || ((uintptr_t)c->pool & 15) || n < 0 || (n > 0 && (!src || !dst)))
@@ -634,6 +638,38 @@ int holo_kv4_pages_free(holo_kv4_pages_t *p, const int *seqs, int n)
             p->set(seqs[i], j, -1);
         }
         p->set_len(seqs[i], 0);
+    }
+    p->end();
+    return 0;
+}
+
+int holo_kv4_pages_trim(holo_kv4_pages_t *p, const int *seqs, const int *rows, int n)
+{
+    if (!p || n < 0 || (n > 0 && (!seqs || !rows))) return rejected("holo_kv4_pages_trim: null argument");
+    std::lock_guard<std::mutex> lk(p->mu);
+    try {
+        std::unordered_set<int> seen;
+        size_t updates = 0;
+        for (int i = 0; i < n; i++) {
+            const int s = seqs[i];
+            if (!p->seq_ok(s) || rows[i] < 0 || !seen.insert(s).second || rows[i] > p->len[s])
+                return rejected("holo_kv4_pages_trim: a sequence outside the cache or given twice, or rows that it has not");
+            updates += (size_t)p->pages_of(s) + 1;
+        }
+        if (!p->open()) return rejected("holo_kv4_pages_trim: under graph capture");
+        p->begin(updates, 0);
+    } catch (const std::bad_alloc &) {
+        return out_of_memory("holo_kv4_pages_trim");
+    }
+    for (int i = 0; i < n; i++) {
+        const int s = seqs[i];
+        if (rows[i] == 0) continue;
+        const int had = p->pages_of(s), keep = (p->len[s] - rows[i] + p->c.page_len - 1) / p->c.page_len;
+        for (int j = keep; j < had; j++) {
+            p->drop(p->entry(s, j));
+            p->set(s, j, -1);
+        }
+        p->set_len(s, p->len[s] - rows[i]);
     }
     p->end();
     return 0;

@@ -111,6 +111,62 @@ __global__ __launch_bounds__(1024) void softmax_k(float *dst, const float *x, in
     for (int i = threadIdx.x; i < n; i += blockDim.x) dst[i] *= inv;
 }
 
+// Each of many rows: softmax(scale (x - max x)), a row of nothing but -infinity zeros.
+// A workgroup takes a row; up to 4 R values a thread stay in registers, longer rows
+// are read again.  V: values of a load (4 where the rows are 16-byte aligned).
+template <int T, int R, int V>
+__global__ __launch_bounds__(T) void softmax_rows_k(float *dst, const float *x, int n, int ldd, int ldx, float scale)
+{
+    __shared__ float scratch[16];
+    typedef float vec __attribute__((ext_vector_type(V)));
+    const float *in = x + (int64_t)blockIdx.x * ldx;
+    float *out = dst + (int64_t)blockIdx.x * ldd;
+    constexpr int C = 4 * R / V;  // loads of a thread
+    const int whole = n / V;      // (V divides n: the caller sees to it)
+    vec v[C];
+    float m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int i = c * T + (int)threadIdx.x;
+        v[c] = i < whole ? ((const vec *)in)[i] : (vec)(-INFINITY);
+#pragma unroll
+        for (int k = 0; k < V; k++) m = fmaxf(m, v[c][k]);
+    }
+    for (int64_t i = (int64_t)C * T + threadIdx.x; i < whole; i += T) {
+        const vec w = ((const vec *)in)[i];
+#pragma unroll
+        for (int k = 0; k < V; k++) m = fmaxf(m, w[k]);
+    }
+    m = block_reduce<true>(m, scratch);
+    const float from = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            v[c][k] = expf((v[c][k] - from) * scale);
+            s += v[c][k];
+        }
+    for (int64_t i = (int64_t)C * T + threadIdx.x; i < whole; i += T) {
+        const vec w = ((const vec *)in)[i];
+#pragma unroll
+        for (int k = 0; k < V; k++) s += expf((w[k] - from) * scale);
+    }
+    s = block_reduce<false>(s, scratch);
+    const float inv = s == 0.f ? 0.f : 1.0f / s;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int i = c * T + (int)threadIdx.x;
+        if (i < whole) ((vec *)out)[i] = v[c] * inv;
+    }
+    for (int64_t i = (int64_t)C * T + threadIdx.x; i < whole; i += T) {
+        vec w = ((const vec *)in)[i];
+#pragma unroll
+        for (int k = 0; k < V; k++) w[k] = expf((w[k] - from) * scale) * inv;
+        ((vec *)out)[i] = w;
+    }
+}
+
 // ---- attention (cuda_ops.cu:1600-1652, 1813-1952, 1960-2096) ------------------------------
 
 __global__ void attention_scores_k(float *dst, const float *Q, const float *K, int seq_len, int kv_len, int hd,
@@ -1883,6 +1939,22 @@ void holo_rms_norm_rows(float *dst, const float *x, const float *weight, int row
     else
         hipLaunchKernelGGL(rms_norm_rows_k, dim3(rows), dim3(256), 0, stream(), dst, x, weight, n, eps);
     HOLO_LAUNCH_CHECK();
+}
+
+int holo_softmax_rows(float *dst, const float *x, int rows, int n, int ldd, int ldx, float scale)
+{
+    if (rows < 0 || n < 0 || (rows > 0 && n > 0 && (!dst || !x || ldd < n || ldx < n || !(scale > 0.f) || scale > 3.402823466e38f))) {
+        HOLO_REJECT("holo_softmax_rows: a null pointer, rows that overlap, or a scale that is not positive and finite");
+        return HOLO_EINVAL;
+    }
+    if (rows == 0 || n == 0) return 0;
+    const bool by4 = (((uintptr_t)dst | (uintptr_t)x) & 15) == 0 && n % 4 == 0 && ldd % 4 == 0 && ldx % 4 == 0;
+    if (by4)
+        hipLaunchKernelGGL((softmax_rows_k<1024, 8, 4>), dim3(rows), dim3(1024), 0, stream(), dst, x, n, ldd, ldx, scale);
+    else
+        hipLaunchKernelGGL((softmax_rows_k<1024, 8, 1>), dim3(rows), dim3(1024), 0, stream(), dst, x, n, ldd, ldx, scale);
+    HOLO_LAUNCH_CHECK();
+    return 0;
 }
 
 void holo_rope_rows(float *q, float *k, int rows, int pos0, int head_dim, int n_heads, int n_kv_heads,

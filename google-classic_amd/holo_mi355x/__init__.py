@@ -200,6 +200,15 @@ _SIGS = {
     "holo_kv4_read": (_I, [_P, _I, _P, _P, _I, _I, _P]),
     "holo_attention_kv4": (_I, [_P, _I, _P, _P, _I, _I, _I, _P]),
     "holo_kv4_copy_pages": (_I, [_P, _P, _P, _I]),
+    # rotary positions of a batch, drafted tokens
+    "holo_softmax_rows": (_I, [_P, _P, _I, _I, _I, _I, _F]),
+    "holo_kv4_append_rope": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _I, _P, _P]),
+    "holo_rope_freqs": (_I, [_P, _P, _P]),
+    "holo_draft_plan": (_I, [_P, _P, _P, _I, _P]),
+    "holo_attention_kv4_draft": (_I, [_P, _I, _P, _P, _I, _I, _I, _P, _I, _P]),
+    "holo_draft_verify": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P]),
+    "holo_kv4_keep": (_I, [_P, _P, _P, _P]),
+    "holo_kv4_pages_trim": (_I, [_P, _P, _P, _I]),
     "holo_kv4_pages_create": (_P, [_P]),
     "holo_kv4_pages_destroy": (None, [_P]),
     "holo_kv4_pages_reserve": (_I, [_P, _P, _P, _I]),
@@ -312,6 +321,21 @@ class KV4(C.Structure):
     """holo_kv4_t (include/holo_forward.h)."""
     _fields_ = [("pool", C.c_void_p), ("table", C.c_void_p), ("len", C.c_void_p)] + [
         (n, C.c_int) for n in ("n_pages", "page_len", "n_layers", "n_kv_heads", "head_dim", "n_seqs", "max_pages")]
+
+
+class Rope(C.Structure):
+    """holo_rope_t (include/holo_forward.h)."""
+    _fields_ = [("freq", C.c_void_p), ("dims", C.c_int), ("interleaved", C.c_int), ("scale", C.c_float)]
+
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BANDS, ROPE_RAMP = range(5)
+DRAFT_CHOSEN, DRAFT_DRAWN, DRAFT_DISTINCT = range(3)
+
+
+class RopeScaling(C.Structure):
+    """holo_rope_scaling_t (include/holo_forward.h)."""
+    _fields_ = [("kind", C.c_int), ("dims", C.c_int), ("base", C.c_double), ("factor", C.c_double),
+                ("low", C.c_double), ("high", C.c_double), ("trained", C.c_int), ("divisors", C.c_void_p)]
 
 
 class HoloError(RuntimeError):

@@ -49,6 +49,13 @@ void holo_embedding_rows(float *dst, const void *embeddings, const int *tokens, 
  * n_kv_heads) (cuda_multi_head_attention, cuda_ops.h:112, per row).           */
 void holo_attention_prefill(float *out, const float *q, const float *k_cache, const float *v_cache, int rows,
                             int pos0, int head_dim, int n_heads, int n_kv_heads);
+/* Each row of n values to softmax(scale (x - max x)): the logits of several tokens
+ * to probabilities, scale 1 / temperature (large for the largest alone).  ldd and
+ * ldx are the floats from one row to the next; dst may be x with the same ld.
+ * Values of -infinity get 0, a row of nothing else is zeros; a row with NaN or
+ * +infinity is NaN.  Returns 0 or HOLO_EINVAL (nothing launched): a scale that is
+ * not positive and finite.  (cuda_softmax takes one row, cuda_ops.h:79.)         */
+int holo_softmax_rows(float *dst, const float *x, int rows, int n, int ldd, int ldx, float scale);
 /* Y[rows][out] = X[rows][in] . W^T for any GEMV type (holo_matmul per row).
  * rows >= 3 with in_dim whole blocks takes the batched MFMA product
  * (holo_matmul_batch) unless `exact` is set.                                  */
@@ -142,6 +149,114 @@ int holo_kv4_read(const holo_kv4_t *c, int layer, float *k, float *v, int ldk, i
  * without memory for its partial sums the hipError_t.                          */
 int holo_attention_kv4(const holo_kv4_t *c, int layer, float *out, const float *q, int ldo, int ldq, int n_heads,
                        const holo_batch_t *b);
+/* ---- rotary positions of a batch ------------------------------------------------------
+ * Pair i of a head's leading `dims` dims turns by t = position * freq[i]: (a, b)
+ * becomes scale * (a cos t - b sin t, a sin t + b cos t), in 64 bits, rounded once;
+ * the other dims pass as they are.                                              */
+typedef struct {
+    const double *freq; /* device, [dims / 2]: radians a position, each pair's (holo_rope_freqs) */
+    int dims;           /* even, 2 .. head_dim */
+    int interleaved;    /* a pair is dims (2 i, 2 i + 1); 0: (i, i + dims / 2), as cuda_rope_apply has it */
+    float scale;        /* 1, or what holo_rope_freqs gives */
+} holo_rope_t;
+
+/* holo_kv4_append of rotated keys, and the queries rotated beside it.  The
+ * cache gets the keys at their rows' places (the last positions of their
+ * sequences) and the values; k_out (NULL: none) the rotated keys as floats, for
+ * holo_attention_packed; q_out the rotated queries.  q_out may be q and k_out k,
+ * with the same ld; otherwise nothing that is written overlaps what is read.  A
+ * row turns by len - r + i (row i of an entry of r rows), or with depth (device,
+ * [rows]) by len - r + depth[row]: rows of a tree.  n_heads 0: no queries.
+ * Rows without a page, or before position 0, are rotated all the same.  0 or
+ * HOLO_EINVAL.  (cuda_rope_apply, cuda_ops.h:117, takes one row.)               */
+int holo_kv4_append_rope(const holo_kv4_t *c, int layer, const holo_rope_t *r, const float *q, const float *k,
+                         const float *v, int ldq, int ldk, int ldv, float *q_out, float *k_out, int ldqo, int ldko,
+                         int n_heads, const int *depth, const holo_batch_t *b);
+
+/* Frequencies, on the host: base^(-2 i / dims), each divided by divisors[i] where
+ * there are any, and for contexts `factor` times the trained one
+ *   PLAIN   as they are (factor and what follows it are not read)
+ *   LINEAR  divided by factor
+ *   BASE    with base * factor^(dims / (dims - 2)) for base
+ *   BANDS   pairs that turn more than `high` times over the `trained` positions as
+ *           they are, those that turn less than `low` times divided by factor,
+ *           between them the mean weighted by (turns - low) / (high - low)
+ *   RAMP    the same, weighted along the pairs' numbers instead, from the one
+ *           that turns `high` times (rounded down) to the one that turns `low`
+ *           times (up); scale becomes 0.1 ln(factor) + 1, otherwise it is 1
+ * freq: host, [dims / 2]; scale may be NULL.  0 or HOLO_EINVAL.                     */
+#define HOLO_ROPE_PLAIN 0
+#define HOLO_ROPE_LINEAR 1
+#define HOLO_ROPE_BASE 2
+#define HOLO_ROPE_BANDS 3
+#define HOLO_ROPE_RAMP 4
+typedef struct {
+    int kind, dims;        /* dims: even, up to 128 (BASE: from 4) */
+    double base;           /* above 1 */
+    double factor;         /* at least 1 */
+    double low, high;      /* 0 < low < high */
+    int trained;           /* positions */
+    const float *divisors; /* host, [dims / 2], positive; NULL: none */
+} holo_rope_scaling_t;
+int holo_rope_freqs(double *freq, float *scale, const holo_rope_scaling_t *s);
+
+/* ---- drafted tokens ------------------------------------------------------------------
+ * A small model drafts what may follow a sequence, the large one runs over all of
+ * it in one step.  An entry's row 0 is then the sequence's last token, the others
+ * the drafted ones: parent[row] (device, [rows]) is the row of the entry that a
+ * row follows, an earlier one, anything else none.  A step:
+ *   holo_kv4_pages_reserve   positions for all rows of the entries
+ *   holo_draft_plan          once
+ *   holo_kv4_append_rope, holo_attention_kv4_draft   in every layer
+ *   holo_softmax_rows, holo_draft_verify             on the rows' logits
+ *   holo_kv4_keep            the rows that stand to the front, every layer
+ *   holo_kv4_pages_trim      the other rows' positions given back
+ * All but the pages' calls can be captured.                                     */
+
+/* Of each row: how many rows it follows up the tree, and itself and those rows as
+ * bits, bit j & 31 of word j / 32 for row j (mask: device, [rows][words]).  max_rows up
+ * to 32 * words, words up to 32.  0 or HOLO_EINVAL.                                */
+int holo_draft_plan(const int *parent, int *depth, uint32_t *mask, int words, const holo_batch_t *b);
+/* holo_attention_kv4 of rows that see the positions before their entry's rows, and
+ * of these the ones whose bits their mask has (any mask, its own row's bit too;
+ * rows past the words have none).  A row that sees nothing gives zeros.  max_rows up
+ * to 32 * words, words up to 32, otherwise as holo_attention_kv4.                 */
+int holo_attention_kv4_draft(const holo_kv4_t *c, int layer, float *out, const float *q, int ldo, int ldq,
+                             int n_heads, const uint32_t *mask, int words, const holo_batch_t *b);
+
+/* Which drafted tokens stand, so that the tokens have the target's distribution.
+ * target and draft: the probabilities of the token behind each row (rows ldt and
+ * ldd floats apart); tokens, parent and u, random numbers in [0, 1), of each
+ * row.  A walk begins at row 0 and judges the rows in order whose parent it is at,
+ * with p and q that row's probabilities, x the judged token, N = 1 and beta = Q = 0:
+ *   DRAWN     the tokens behind a row were drawn from its q, each by itself.  It
+ *             stands if u q(x) N < max(p(x) - beta q(x), 0) (1 - Q); else beta += N / (1 - Q),
+ *             N = sum max(p - beta q, 0)
+ *   DISTINCT  they were drawn without repeats: and Q += q(x)
+ *   CHOSEN    they were not drawn (the most probable ones, say; draft is not read).
+ *             It stands if u N < p(x), p(x) = 0 for a token refused here before; else
+ *             N -= p(x)
+ * A row that stands is where the walk goes on, with N = 1 and beta = Q = 0.
+ * path (device, [rows]) gets the entry's rows that stand, row 0 first, then -1;
+ * n_path[s] how many; next[s] the token behind the last of them: the first x at which the
+ * sum of w(0 .. x) passes u of row 0 times the sum of all, w = max(p - beta q, 0), or p
+ * without the refused tokens (no weight at all: the target's most probable token).  Sums are
+ * in 64 bits.  target's rows sum to 1; values that are negative or no finite
+ * numbers count as 0.  Tokens outside 0 .. vocab - 1 never stand.  An entry without
+ * rows: n_path 0, next -1.  vocab up to 2^24, max_rows up to 1024.  0 or HOLO_EINVAL. */
+#define HOLO_DRAFT_CHOSEN 0
+#define HOLO_DRAFT_DRAWN 1
+#define HOLO_DRAFT_DISTINCT 2
+int holo_draft_verify(int *path, int *n_path, int *next, const float *target, const float *draft, int ldt, int ldd,
+                      int vocab, const int *tokens, const int *parent, const float *u, int mode, const holo_batch_t *b);
+/* Of each entry, row path[i] to the place of row i for i < n_path[s], keys and
+ * values, every layer: what holo_kv4_append_rope would have stored of these rows
+ * alone.  path rises (device, [rows], as holo_draft_verify leaves it); an entry of
+ * it outside the rows, or a place without a page, moves nothing.  What the other positions
+ * hold stays.  The pages written must not be shared (holo_kv4_pages_reserve sees to it).
+ * 0 or HOLO_EINVAL.                                                             */
+int holo_kv4_keep(const holo_kv4_t *c, const int *path, const int *n_path, const holo_batch_t *b);
+
 /* Page dst[i] becomes a copy of page src[i], every layer (host arrays).
  * HOLO_EINVAL, and nothing copied, for a page outside the pool, a page written
  * twice, or one that is read and written.                                      */
@@ -164,6 +279,9 @@ int holo_kv4_pages_reserve(holo_kv4_pages_t *p, const int *seqs, const int *rows
 /* The empty sequence dst[i] becomes a copy of src[i], sharing its pages.  Entry
  * by entry: a src may be an earlier dst.                                       */
 int holo_kv4_pages_fork(holo_kv4_pages_t *p, const int *src, const int *dst, int n);
+/* The last rows[i] positions of sequence seqs[i] (a sequence once) given back, and
+ * the pages that hold no others.  HOLO_EINVAL for more than it has.             */
+int holo_kv4_pages_trim(holo_kv4_pages_t *p, const int *seqs, const int *rows, int n);
 /* Sequences emptied; pages that no other sequence shares are free again.       */
 int holo_kv4_pages_free(holo_kv4_pages_t *p, const int *seqs, int n);
 /* The pages in use moved to the front of the pool: 0 .. used - 1.              */
