@@ -228,7 +228,7 @@ def test_rotation_leaves_rows_past_max_rows_and_passes_bad_values(holo):
         assert (got[6:9] == -9.0).all()
         assert np.array_equal(np.isfinite(got[kept]), np.isfinite(want[kept]))
         ok = np.isfinite(want[kept])
-            assert (np.abs(got[kept][ok] - want[kept][ok]) <= 2.0 ** -24 * np.abs(want[kept][ok]) + 1e-9).all()
+        assert (np.abs(got[kept][ok] - want[kept][ok]) <= 2.0 ** -24 * np.abs(want[kept][ok]) + 1e-9).all()
     for i in kept:
         s, p = (0, 11 + i) if i < 9 else (1, i - 9)
         with np.errstate(invalid="ignore"):
