@@ -79,26 +79,7 @@ struct Kv4Attn {
     int ldo, ldq, n_heads;
     int splits;  // the most ranges that a sequence is cut into
     int ctiles;  // tiles of 16 columns that max_rows rows have
-    // drafted rows (attn_kv4_draft.hip): bit j of row i's words: it sees row j of its entry
-    const uint32_t *mask;
-    int words;
 };
-
-// Which of tile t's positions a drafted row sees, one bit each: those before the
-// entry's rows (the first at position `from`), and the rows that its words name.
-__device__ __forceinline__ uint32_t draft_sees(const uint32_t *words, int n_words, int t, int from, int len)
-{
-    const int at = 32 * t - from, left = len - 32 * t;  // the tile's first position among the rows
-    uint32_t bits;
-    if (at <= -32) bits = 0xFFFFFFFFu;
-    else if (at < 0) bits = ((1u << -at) - 1u) | words[0] << -at;
-    else {
-        const int w = at >> 5, s = at & 31;
-        bits = w < n_words ? words[w] >> s : 0u;
-        if (s && w + 1 < n_words) bits |= words[w + 1] << (32 - s);
-    }
-    return left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1u) : 0u;
-}
 
 // The partial sums of an entry's row and head, range after range: hd sums, the
 // maximum they are relative to and the probabilities' sum.
@@ -114,8 +95,8 @@ __device__ __forceinline__ int range_of(const Kv4Attn &a, int n)
 }
 
 // Column c of an entry and KV head: row c / G, query head kvh * G + c % G.
-// Waves: W; the columns of a workgroup: 16.  DRAFT: rows see what their masks say.
-template <int NB, int W, bool DRAFT = false>
+// Waves: W; the columns of a workgroup: 16.
+template <int NB, int W>
 __global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
 {
     constexpr int HD = 32 * NB, OS = HD + 4;
@@ -131,7 +112,7 @@ __global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
     // the tiles that the tile's last row sees, in ranges
     const int last_row = (min(c0 + 16, ncols) - 1) / G, first_row = c0 / G;
     const int from = e.len - e.rows;
-    const int see = DRAFT ? e.len : max(from + last_row + 1, 0);  // positions the last row sees
+    const int see = max(from + last_row + 1, 0);  // positions the last row sees
     const int ntiles = too_long ? 0 : (see + 31) >> 5;
     const int chunk = range_of(a, ntiles), t0 = blockIdx.x * chunk, t1 = min(t0 + chunk, ntiles);
     if (t0 >= ntiles && blockIdx.x > 0) return;
@@ -140,8 +121,7 @@ __global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
     const int col = min(c0 + r, ncols - 1);  // past the last: the last again
     const int row = col / G, head = kvh * G + col % G;
     const int qpos = from + row;               // the column sees positions 0 .. qpos
-    const int all = DRAFT ? from - 1 : from + first_row;  // positions 0 .. all are seen by every column
-    const uint32_t *words = DRAFT ? a.mask + (int64_t)(e.first + row) * a.words : nullptr;
+    const int all = from + first_row;          // positions 0 .. all are seen by every column
 
     // q of the column: dims 8 (NB g + j) .. + 7 in step j, scaled to [2^13, 2^14)
     h8 qh[NB], ql[NB];
@@ -209,13 +189,9 @@ __global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
     int poison = 0;  // by block of dims: this lane's positions have a NaN that the column sees
     auto mask = [&](int t, bool there) {
         const int sees = (there ? qpos : -1) - 32 * t, end = there ? e.len - 32 * t : 0;
-        uint32_t bits = 0;
-        if constexpr (DRAFT)
-            if (there) bits = draft_sees(words, a.words, t, from, e.len);
-        auto hidden = [&](int i) { return DRAFT ? !(bits >> v_pos(g, i) & 1u) : v_pos(g, i) > sees; };
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (hidden(i)) s[i >> 2][i & 3] = -INFINITY;
+            if (v_pos(g, i) > sees) s[i >> 2][i & 3] = -INFINITY;
         uint32_t keep[4];  // of the lane's positions, two a register
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -240,7 +216,7 @@ __global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const bool is = d[i] != d[i];
-                    nan |= is && !hidden(i);
+                    nan |= is && v_pos(g, i) <= sees;
                     if (is && v_pos(g, i) > all_see) d[i] = (_Float16)0.f;
                 }
                 xv.s[b] = __builtin_bit_cast(u4, d);
@@ -361,25 +337,15 @@ __global__ __launch_bounds__(64 * W, NB == 3 ? 2 : 3) void attn_kv4_k(Kv4Attn a)
     }
 }
 
-// Joins the ranges of a row and head, in range order: groups of HD / 4 lanes take
-// every 256 / (HD / 4)-th range, four dims a lane, and meet in LDS in group order.
-template <int NB, bool DRAFT = false>
-__global__ __launch_bounds__(256) void attn_kv4_join_k(Kv4Attn a)
+// Joins the n ranges of a row and head, in range order, their partial sums `stride`
+// floats apart: groups of HD / 4 lanes take every 256 / (HD / 4)-th range, four dims a
+// lane, and meet in LDS in group order.
+template <int NB>
+__device__ __forceinline__ void kv4_join(const float *pp, int64_t stride, int n, float *out)
 {
     constexpr int HD = 32 * NB, D = HD / 4, GR = 256 / D, R = 4;
     __shared__ __align__(16) float lo_[GR][HD];
     __shared__ float lm[GR], ll[GR];
-    const Kv4Entry e = kv4_entry(a.c, a.b, blockIdx.z);
-    const int h = blockIdx.x, row = blockIdx.y;
-    if (row >= e.take || e.len > a.b.max_len) return;
-    const int G = a.n_heads / a.c.n_kv_heads;
-    // the ranges of the row's tile of columns, as the workgroups above have it
-    const int c0 = (row * G + h % G) & ~15, last_row = (min(c0 + 16, e.take * G) - 1) / G;
-    const int ntiles = ((DRAFT ? e.len : max(e.len - e.rows + last_row + 1, 0)) + 31) >> 5;
-    const int chunk = range_of(a, ntiles), n = (ntiles + chunk - 1) / chunk;
-    if (n <= 1) return;
-    const int64_t at = e.first + row;
-    const float *pp = partial(a, blockIdx.z, row, h, HD);
     const int g = threadIdx.x / D, d = 4 * (threadIdx.x % D);
     float M = -FLT_MAX, L = 0.f;
     f4 O = f4{};
@@ -389,7 +355,7 @@ __global__ __launch_bounds__(256) void attn_kv4_join_k(Kv4Attn a)
             f4 x[R];
 #pragma unroll
             for (int i = 0; i < R; i++) {
-                const float *p = pp + (int64_t)min(s0 + GR * i, n - 1) * (HD + 4);
+                const float *p = pp + (int64_t)min(s0 + GR * i, n - 1) * stride;
                 ml[i] = *(const f2 *)(p + HD);
                 x[i] = *(const f4 *)(p + d);
             }
@@ -425,7 +391,25 @@ __global__ __launch_bounds__(256) void attn_kv4_join_k(Kv4Attn a)
         L = fmaf(f, ll[i], L);
         O += f * *(const f4 *)&lo_[i][d];
     }
-    *(f4 *)(a.out + at * a.ldo + (int64_t)h * HD + d) = O * (L == 0.f ? 0.f : 1.0f / L);
+    *(f4 *)(out + d) = O * (L == 0.f ? 0.f : 1.0f / L);
+}
+
+template <int NB>
+__global__ __launch_bounds__(256) void attn_kv4_join_k(Kv4Attn a)
+{
+    constexpr int HD = 32 * NB;
+    const Kv4Entry e = kv4_entry(a.c, a.b, blockIdx.z);
+    const int h = blockIdx.x, row = blockIdx.y;
+    if (row >= e.take || e.len > a.b.max_len) return;
+    const int G = a.n_heads / a.c.n_kv_heads;
+    // the ranges of the row's tile of columns, as the workgroups above have it
+    const int c0 = (row * G + h % G) & ~15, last_row = (min(c0 + 16, e.take * G) - 1) / G;
+    const int ntiles = (max(e.len - e.rows + last_row + 1, 0) + 31) >> 5;
+    const int chunk = range_of(a, ntiles), n = (ntiles + chunk - 1) / chunk;
+    if (n <= 1) return;
+    const int64_t at = e.first + row;
+    const float *pp = partial(a, blockIdx.z, row, h, HD);
+    kv4_join<NB>(pp, HD + 4, n, a.out + at * a.ldo + (int64_t)h * HD);
 }
 
 // Ranges: one where a sequence has few tiles (700 positions of 32 sequences, a

@@ -82,7 +82,7 @@ extern "C" int holo_attention_kv4(const holo_kv4_t *c, int layer, float *out, co
     }
     if (b->rows == 0 || b->n_seqs == 0) return 0;
     const int64_t dim = (int64_t)n_heads * c->head_dim;
-    Kv4Attn a{kv4_view(c, layer), *b, out, nullptr, q, ldo, ldq, n_heads, 0, 0, nullptr, 0};
+    Kv4Attn a{kv4_view(c, layer), *b, out, nullptr, q, ldo, ldq, n_heads, 0, 0};
     a.b.max_rows = b->max_rows < b->rows ? b->max_rows : b->rows;
     const int64_t cols = (int64_t)a.b.max_rows * (n_heads / c->n_kv_heads);
     if (!rows_ok(q, ldq, dim) || !rows_ok(out, ldo, dim) || b->max_len < 0 || b->max_len > 0x7FFFF000 ||
