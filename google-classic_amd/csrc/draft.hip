@@ -2,6 +2,7 @@
 // which of them stand against the target's probabilities.
 #include "block_reduce.h"
 #include "kv4.h"
+#include "stream_scratch.h"
 
 #include <float.h>
 
@@ -53,6 +54,19 @@ __global__ __launch_bounds__(1024) void draft_plan_k(const int *parent, int *dep
 }
 
 // ---- verification ----------------------------------------------------------------------------
+//
+// Probabilities are given, so that what stands and the next token do not depend on how a
+// kernel rounds an exponential: products and sums of them are in 64 bits, where two orders
+// of a sum differ by 10^-16 and a token's border is hit once in 10^11 calls.  After
+// refusals the weights left are max(p - beta q, 0) in closed form, so that a sum N over the row is
+// all that a refusal costs.
+//
+// What bounds it: latency.  64 chains of 5 rows, 32000 tokens, 16.4 MB of the rows that the
+// walks end at (3.4 us at a large copy's rate): 12.8-13.1 us, two launches of 5 and 4.4 with loads
+// that depend on each other (rows, tokens, probabilities; then the row); with one workgroup an entry for
+// all of it 42.  16 trees of up to 26 rows 28-32 (78): the second launch goes from refusal to
+// refusal, some 4 us each, half of it 64-bit arithmetic; with the row's probabilities kept in registers
+// the compiler spills them (50-57).
 
 struct Verify {
     int *path, *n_path, *next;
@@ -61,6 +75,8 @@ struct Verify {
     const int *tokens, *parent;
     const float *u;
     int block;  // tokens of a partial sum, a multiple of 256
+    struct WalkState *states;  // of each entry: where its walk stands, and the sums of the weights there
+    double *sums;
 };
 
 constexpr int kVerifyThreads = 1024, kVerifyWaves = kVerifyThreads / 64, kVerifySums = 2048;
@@ -92,23 +108,161 @@ __device__ __forceinline__ double weight(float p, float q, double beta)
     return w > 0.0 ? w : 0.0;
 }
 
-// What the walk has reached, and the weights that it wants the sums of.
-struct VerifyStep {
-    double beta;
-    int node, refused;  // refused: tokens, of a chosen draft
-    bool sum, end;
+// Where a walk stands (the formulas: holo_forward.h).
+struct WalkState {
+    double left, beta, gone;  // N, beta, Q
+    int node, last, count;    // the row that it is at, the row judged last, rows that stand
+    int asks;                 // the row judged last is refused, another follows, and N is wanted for it
 };
 
-// An entry's walk (the formulas: holo_forward.h) by one workgroup.  The first wave
-// judges, 64 rows in its lanes: what a row needs of the two distributions depends on
-// its parent alone and is loaded ahead.  Where the sum of a whole row of weights is
-// needed, all waves sum blocks of tokens, in 64 bits; the same sums then lead to the
-// next token's block.  Every sum has one order.
+// A walk over an entry's rows by one wave, 64 rows in its lanes: what a row needs of
+// the two distributions depends on its parent alone and is loaded ahead.
+struct Walk {
+    const Verify &a;
+    int first, take, lane;
+    WalkState s;
+    int base = -1, up = -1, tok = -1;  // the lanes' rows: base + lane
+    float p = 0.f, q = 0.f, u = 0.f;
+
+    __device__ __forceinline__ Walk(const Verify &a, int first, int take, int lane) : a(a), first(first), take(take), lane(lane)
+    {
+        s = WalkState{1.0, 0.0, 0.0, 0, 0, 1, 0};
+    }
+    __device__ __forceinline__ bool drawn() const { return a.mode != HOLO_DRAFT_CHOSEN; }
+    __device__ __forceinline__ void load_rows(int at)
+    {
+        base = at;
+        const int i = at + lane;
+        up = i > 0 && i < take ? a.parent[first + i] : -1;
+        if (up >= i) up = -1;
+        tok = -1;
+        p = q = 0.f;
+        if (up < 0) return;
+        tok = a.tokens[first + i];
+        u = a.u[first + i];
+        if (tok < 0 || tok >= a.vocab) {
+            tok = -1;
+            return;
+        }
+        p = a.target[(int64_t)(first + up) * a.ldt + tok];
+        if (drawn()) q = a.draft[(int64_t)(first + up) * a.ldd + tok];
+    }
+    // The next row behind the last one whose parent is the node; -1: none.
+    __device__ __forceinline__ int next_row()
+    {
+        for (int at = (s.last + 1) & ~63; at < take; at += 64) {
+            if (at != base) load_rows(at);
+            const uint64_t hit = __ballot(up == s.node && at + lane > s.last);
+            if (hit) return at + __ffsll((unsigned long long)hit) - 1;
+        }
+        return -1;
+    }
+    // Chosen: whether row j's token is that of an earlier row behind the node, which was refused.
+    __device__ __forceinline__ bool again(int j, int t)
+    {
+        bool same = __any(up == s.node && base + lane < j && tok == t);
+        for (int at = 0; at < base && !same; at += 64)
+            same = __any(a.parent[first + at + lane] == s.node && at + lane > s.node && a.tokens[first + at + lane] == t);
+        return same;
+    }
+    // Judges rows until N is wanted (asks) or none is left; stood(i, row): row i of the path.
+    template <typename F>
+    __device__ __forceinline__ void go(F stood)
+    {
+        s.asks = 0;
+        for (int j; (j = next_row()) >= 0;) {
+            s.last = j;
+            const int t = __shfl(tok, j & 63, 64);
+            const float pj = __shfl(p, j & 63, 64), qj = __shfl(q, j & 63, 64), uj = __shfl(u, j & 63, 64);
+            const double qx = probability(qj);
+            double px = weight(pj, qj, s.beta);
+            bool stands;
+            if (drawn()) {
+                stands = (double)uj * qx * s.left < px * (1.0 - s.gone);
+            } else {
+                if (t >= 0 && again(j, t)) px = 0.0;
+                stands = (double)uj * s.left < px;
+            }
+            if (stands) {
+                stood(s.count, j);
+                s = WalkState{1.0, 0.0, 0.0, j, j, s.count + 1, 0};
+            } else if (!drawn()) {
+                s.left -= px;
+            } else if (t >= 0 && s.gone < 1.0) {
+                s.beta += s.left / (1.0 - s.gone);
+                if (a.mode == HOLO_DRAFT_DISTINCT) s.gone += qx;
+                s.asks = next_row() >= 0;  // (behind the last one the sum is part of finding the next token)
+                return;
+            }
+        }
+    }
+};
+
+// The sums of the weights of blocks e, e + stride, .. (U of them), by a wave: the loads
+// of all of them under way at once.
+template <int U>
+__device__ __forceinline__ void block_sums(const Verify &a, const float *p, const float *q, double beta, int e, int stride, int lane,
+                                           double *to, int nsums)
+{
+    double sum[U] = {};
+    for (int o = lane; o < a.block; o += 256) {
+        float x[U][4], y[U][4];
+#pragma unroll
+        for (int i = 0; i < U; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t at = (uint32_t)((e + i * stride) * a.block + o + 64 * k);  // (vocab up to 2^24)
+                x[i][k] = at < (uint32_t)a.vocab ? p[at] : 0.f;
+                y[i][k] = at < (uint32_t)a.vocab && beta != 0.0 ? q[at] : 0.f;
+            }
+#pragma unroll
+        for (int i = 0; i < U; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) sum[i] += weight(x[i][k], y[i][k], beta);
+    }
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+        const double s = wave_sum(sum[i]);
+        if (lane == 0 && e + i * stride < nsums) to[e + i * stride] = s;
+    }
+}
+
+// The start of every entry's walk, up to where a sum over a row is wanted, which for a
+// chain is where it ends: each of an entry's workgroups walks by itself and sums some of
+// the row's blocks, the first one writes down where the walk stands.
+__global__ __launch_bounds__(256) void draft_verify_start_k(Verify a, holo_batch_t b)
+{
+    __shared__ WalkState state;
+    const int e = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int first, take;
+    batch_rows(b, e, first, take);
+    if (take <= 0) return;
+    if (wave == 0) {
+        Walk w(a, first, take, lane);
+        const bool writes = blockIdx.x == 0 && lane == 0;
+        if (writes) a.path[first] = 0;
+        w.go([&](int i, int row) {
+            if (writes) a.path[first + i] = row;
+        });
+        if (writes) a.states[e] = w.s;
+        if (lane == 0) state = w.s;
+    }
+    __syncthreads();
+    const WalkState s = state;
+    const float *p = a.target + (int64_t)(first + s.node) * a.ldt;
+    const float *q = a.mode != HOLO_DRAFT_CHOSEN ? a.draft + (int64_t)(first + s.node) * a.ldd : p;
+    const int nsums = (a.vocab + a.block - 1) / a.block;
+    double *sums = a.sums + (int64_t)e * nsums;
+    for (int i = 4 * blockIdx.x + wave; i < nsums; i += 4 * gridDim.x) block_sums<1>(a, p, q, s.beta, i, 1, lane, sums, nsums);
+}
+
+// The rest, a workgroup an entry: more rows behind a refused one (the branches of a
+// tree), and the next token.  Sums are in 64 bits, each in one order.
 __global__ __launch_bounds__(kVerifyThreads) void draft_verify_k(Verify a, holo_batch_t b)
 {
     __shared__ double sums[kVerifySums];
     __shared__ int refused_tok[1024];
-    __shared__ VerifyStep step;
+    __shared__ WalkState state;
     int first, take;
     batch_rows(b, blockIdx.x, first, take);
     if (take <= 0) {
@@ -121,40 +275,7 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_k(Verify a, holo_
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool drawn = a.mode != HOLO_DRAFT_CHOSEN;
     const int nsums = (a.vocab + a.block - 1) / a.block, per = (nsums + 63) / 64;
-
-    // the first wave's: row judged last, rows that stand, N, beta, Q
-    int node = 0, last = 0, count = 1, refused = 0;
-    double left = 1.0, beta = 0.0, gone = 0.0;
-    bool summed = false;  // sums are of this node and beta
-    // its lanes' rows: base + lane
-    int base = -1, r_up = -1, r_tok = -1;
-    float r_p = 0.f, r_q = 0.f, r_u = 0.f;
-    auto load_rows = [&](int at) {
-        base = at;
-        const int i = at + lane;
-        r_up = i > 0 && i < take ? a.parent[first + i] : -1;
-        if (r_up >= i) r_up = -1;
-        r_tok = -1;
-        r_p = r_q = 0.f;
-        if (r_up < 0) return;
-        r_tok = a.tokens[first + i];
-        r_u = a.u[first + i];
-        if (r_tok < 0 || r_tok >= a.vocab) {
-            r_tok = -1;
-            return;
-        }
-        r_p = a.target[(int64_t)(first + r_up) * a.ldt + r_tok];
-        if (drawn) r_q = a.draft[(int64_t)(first + r_up) * a.ldd + r_tok];
-    };
-    // The next row behind `last` whose parent is the node; -1: none.
-    auto next_row = [&]() {
-        for (int at = (last + 1) & ~63; at < take; at += 64) {
-            if (at != base) load_rows(at);
-            const uint64_t hit = __ballot(r_up == node && at + lane > last);
-            if (hit) return at + __ffsll((unsigned long long)hit) - 1;
-        }
-        return -1;
-    };
+    for (int i = threadIdx.x; i < nsums; i += kVerifyThreads) sums[i] = a.sums[(int64_t)blockIdx.x * nsums + i];
     // Sum of all blocks; upto: of those up to the end of this lane's.
     auto total = [&](double &upto) {
         double s = 0.0;
@@ -162,104 +283,61 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_k(Verify a, holo_
         upto = wave_scan(s, lane);
         return __shfl(upto, 63, 64);
     };
-    // Judges rows until a sum is needed (true) or none is left.
-    auto walk = [&]() {
-        for (int j; (j = next_row()) >= 0;) {
-            last = j;
-            const int tok = __shfl(r_tok, j & 63, 64);
-            const float p = __shfl(r_p, j & 63, 64), q = __shfl(r_q, j & 63, 64), u = __shfl(r_u, j & 63, 64);
-            const double qx = probability(q);
-            double px = weight(p, drawn ? q : 0.f, beta);
-            bool stands;
-            if (drawn) {
-                stands = (double)u * qx * left < px * (1.0 - gone);
-            } else {
-                bool again = false;  // a token refused at this node before: nothing is left of it
-                for (int i = lane; i < refused; i += 64) again |= refused_tok[i] == tok;
-                if (__any(again)) px = 0.0;
-                stands = (double)u * left < px;
-            }
-            if (stands) {
-                if (lane == 0) a.path[first + count] = j;
-                count++;
-                node = j;
-                left = 1.0;
-                beta = gone = 0.0;
-                refused = 0;
-                summed = false;
-            } else if (!drawn) {
-                if (lane == 0) refused_tok[refused] = tok;
-                wave_lds_fence();
-                refused++;
-                left -= px;
-            } else if (tok >= 0 && gone < 1.0) {
-                beta += left / (1.0 - gone);
-                if (a.mode == HOLO_DRAFT_DISTINCT) gone += qx;
-                return true;
-            }
-        }
-        return false;
-    };
 
-    if (threadIdx.x == 0) a.path[first] = 0;
-    for (;;) {
-        if (wave == 0) {
-            const bool more = walk();
-            if (lane == 0) step = VerifyStep{beta, node, refused, more || !summed, !more};
-        }
-        __syncthreads();
-        const VerifyStep s = step;
-        const float *p = a.target + (int64_t)(first + s.node) * a.ldt;
-        const float *q = drawn ? a.draft + (int64_t)(first + s.node) * a.ldd : p;
-        const double w = drawn ? s.beta : 0.0;
-        if (s.sum) {
-            constexpr int U = 4;
-            for (int e = wave; e < nsums; e += U * kVerifyWaves) {
-                double sum[U] = {};
-                for (int o = lane; o < a.block; o += 256) {
-                    float x[U][4], y[U][4];
-#pragma unroll
-                    for (int i = 0; i < U; i++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const int64_t at = (int64_t)(e + i * kVerifyWaves) * a.block + o + 64 * k;
-                            x[i][k] = at < a.vocab ? p[at] : 0.f;
-                            y[i][k] = at < a.vocab && w != 0.0 ? q[at] : 0.f;
-                        }
-#pragma unroll
-                    for (int i = 0; i < U; i++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) sum[i] += weight(x[i][k], y[i][k], w);
-                }
-#pragma unroll
-                for (int i = 0; i < U; i++) {
-                    sum[i] = wave_sum(sum[i]);
-                    if (lane == 0 && e + i * kVerifyWaves < nsums) sums[e + i * kVerifyWaves] = sum[i];
-                }
-            }
-        }
-        __syncthreads();
-        if (s.end) break;
+    Walk w(a, first, take, lane);
+    w.s = a.states[blockIdx.x];
+    __syncthreads();
+    const float *p, *q;
+    auto rows = [&]() {
+        p = a.target + (int64_t)(first + w.s.node) * a.ldt;
+        q = drawn ? a.draft + (int64_t)(first + w.s.node) * a.ldd : p;
+    };
+    while (w.s.asks) {  // (the same for every wave)
+        const int node = w.s.node;
+        const double beta = w.s.beta;
         if (wave == 0) {
             double upto;
-            left = total(upto);
-            summed = true;
+            w.s.left = total(upto);
+            w.go([&](int i, int row) {
+                if (lane == 0) a.path[first + i] = row;
+            });
+            if (lane == 0) state = w.s;
         }
+        __syncthreads();
+        if (wave != 0) w.s = state;
+        if (w.s.node == node && w.s.beta == beta) break;  // sums are of these
+        rows();
+        constexpr int U = 2;
+        for (int e = wave; e < nsums; e += U * kVerifyWaves)
+            block_sums<U>(a, p, q, w.s.beta, e, kVerifyWaves, lane, sums, nsums);
+        __syncthreads();
     }
-
-    // Chosen: blocks with refused tokens once more, without them.
-    const VerifyStep s = step;
-    const float *p = a.target + (int64_t)(first + s.node) * a.ldt;
-    const float *q = drawn ? a.draft + (int64_t)(first + s.node) * a.ldd : p;
-    auto weight_at = [&](int64_t x) {
-        if (x >= a.vocab) return 0.0;
-        for (int i = 0; i < s.refused; i++)
-            if (refused_tok[i] == x) return 0.0;
-        return weight(p[x], s.beta != 0.0 ? q[x] : 0.f, s.beta);
+    rows();
+    // Chosen: every row behind the node was refused; blocks with such tokens once more, without them.
+    int refused = 0;
+    if (!drawn) {
+        if (wave == 0) {
+            for (int at = 0; at < take; at += 64) {
+                const int i = at + lane;
+                const bool is = i > w.s.node && i < take && a.parent[first + i] == w.s.node;
+                const uint64_t hits = __ballot(is);
+                if (is) refused_tok[refused + __popcll(hits & ((1ull << lane) - 1))] = a.tokens[first + i];
+                refused += __popcll(hits);
+            }
+            if (lane == 0) state.count = refused;
+        }
+        __syncthreads();
+        refused = state.count;
+    }
+    auto weight_at = [&](int64_t t) {
+        if (t >= a.vocab) return 0.0;
+        for (int i = 0; i < refused; i++)
+            if (refused_tok[i] == t) return 0.0;
+        return weight(p[t], w.s.beta != 0.0 ? q[t] : 0.f, w.s.beta);
     };
-    for (int r = wave; r < s.refused; r += kVerifyWaves) {
-        const int e = refused_tok[r] / a.block;
-        if (refused_tok[r] < 0) continue;
+    for (int r = wave; r < refused; r += kVerifyWaves) {
+        const int t = refused_tok[r], e = t / a.block;
+        if (t < 0 || t >= a.vocab) continue;
         double sum = 0.0;
         for (int o = lane; o < a.block; o += 64) sum += weight_at((int64_t)e * a.block + o);
         sum = wave_sum(sum);
@@ -267,7 +345,7 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_k(Verify a, holo_
     }
     __syncthreads();
     if (wave != 0) return;
-    for (int i = count + lane; i < take; i += 64) a.path[first + i] = -1;
+    for (int i = w.s.count + lane; i < take; i += 64) a.path[first + i] = -1;
     double upto;
     const double all = total(upto), at = (double)a.u[first] * all;
     int token = -1;
@@ -286,8 +364,8 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_k(Verify a, holo_
             if (run + sums[i] > at) break;
         }
         for (int o = 0; o < a.block; o += 64) {
-            const int64_t x = (int64_t)e * a.block + o + lane;
-            const double v = weight_at(x), to = run + wave_scan(v, lane);
+            const int64_t t = (int64_t)e * a.block + o + lane;
+            const double v = weight_at(t), to = run + wave_scan(v, lane);
             const uint64_t pos = __ballot(v > 0.0), in = __ballot(to > at) & pos;
             if (pos) token = e * a.block + o + (in ? __ffsll((unsigned long long)in) - 1 : 63 - __clzll((long long)pos));
             if (in) break;
@@ -296,23 +374,23 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_k(Verify a, holo_
     } else {
         // nothing weighs: the target's most probable token, the lowest of equals
         float best = -FLT_MAX;
-        for (int x = lane; x < a.vocab; x += 64)
-            if (p[x] > best || (token < 0 && p[x] == p[x])) {
-                best = p[x];
-                token = x;
+        for (int t = lane; t < a.vocab; t += 64)
+            if (p[t] > best || (token < 0 && p[t] == p[t])) {
+                best = p[t];
+                token = t;
             }
         for (int off = 32; off > 0; off >>= 1) {
             const float v = __shfl_xor(best, off, 64);
-            const int x = __shfl_xor(token, off, 64);
-            if (x >= 0 && (token < 0 || v > best || (v == best && x < token))) {
+            const int t = __shfl_xor(token, off, 64);
+            if (t >= 0 && (token < 0 || v > best || (v == best && t < token))) {
                 best = v;
-                token = x;
+                token = t;
             }
         }
         token = max(token, 0);
     }
     if (lane == 0) {
-        a.n_path[blockIdx.x] = count;
+        a.n_path[blockIdx.x] = w.s.count;
         a.next[blockIdx.x] = token;
     }
 }
@@ -362,7 +440,18 @@ int holo_draft_verify(int *path, int *n_path, int *next, const float *target, co
         return HOLO_EINVAL;
     }
     const int block = (int)(((int64_t)vocab + 256 * kVerifySums - 1) / (256 * kVerifySums)) * 256;
-    const Verify a{path, n_path, next, target, draft, ldt, ldd, vocab, mode, tokens, parent, u, block};
+    const int nsums = (vocab + block - 1) / block;
+    const size_t told = (size_t)b->n_seqs * sizeof(WalkState);
+    const StreamScratch scratch(told + (size_t)b->n_seqs * nsums * sizeof(double));
+    if (!scratch.get()) {
+        latch_error((int)hipErrorOutOfMemory, "holo_draft_verify: sums", __FILE__, __LINE__);
+        return (int)hipErrorOutOfMemory;
+    }
+    const Verify a{path,   n_path, next,  target, draft, ldt,  ldd, vocab, mode,
+                   tokens, parent, u,     block,  (WalkState *)scratch.get(), (double *)((uint8_t *)scratch.get() + told)};
+    const int want = 2048 / b->n_seqs, most = (nsums + 3) / 4, parts = want < 1 ? 1 : want < most ? want : most;
+    hipLaunchKernelGGL(draft_verify_start_k, dim3(parts, b->n_seqs), dim3(256), 0, stream(), a, v);
+    HOLO_LAUNCH_CHECK();
     hipLaunchKernelGGL(draft_verify_k, dim3(b->n_seqs), dim3(kVerifyThreads), 0, stream(), a, v);
     HOLO_LAUNCH_CHECK();
     return 0;
