@@ -135,6 +135,12 @@ __global__ __launch_bounds__(256) void kv4_read_k(Kv4View c, holo_batch_t b, flo
 // goes into one before it writes any of it, and no later source is among what
 // earlier tiles wrote.  A thread makes whole words: the keys of a (position, lane
 // group), the VW dims of eight positions' values.
+//
+// What bounds it: one sequence, 32 layers of 8 heads, four rows moved 5.2-5.5 us, a chain of
+// lengths, path, pages and words, and code that a CU has not run yet.  64 sequences 28 us: 16384
+// workgroups, four to a place on the chip, each that chain; the bytes (28 MB read, 28
+// written: pieces of 64, where the rows themselves are 9.4 and 9.4) would take 11.  Two heads
+// a workgroup 30.5 and 7.5, four 42 and 11.7; loads without branches 31-37.
 template <int NB>
 __global__ __launch_bounds__(NB == 3 ? 192 : 128) void kv4_keep_k(Kv4View c, holo_batch_t b, const int *path,
                                                                  const int *n_path)

@@ -3,6 +3,7 @@
 #include "kv4_quant.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace holo {
 
@@ -14,20 +15,47 @@ struct RopeRows {
     const int *depth;
 };
 
-// Query heads of a workgroup.
-constexpr int kRopeHeads = 4;
+// Query heads of a workgroup (one: 43.1 us for the prompts below with the read back; two
+// 39.7, four 46.2).
+constexpr int kRopeHeads = 2;
 
-// A workgroup takes the rows of one tile of positions, one KV head and up to four of
+// The sine and cosine of position * freq, times the scale.  half_turns: of the freq.
+__device__ __forceinline__ void turn_by(double position, double half_turns, float scale, double &cs, double &sn)
+{
+    double t = position * half_turns;
+    t -= 2.0 * rint(0.5 * t);
+    sincospi(t, &sn, &cs);
+    cs *= scale;
+    sn *= scale;
+}
+
+__device__ __forceinline__ void turn_pair(float &x, float &y, double cs, double sn)
+{
+    const float u = (float)(x * cs - y * sn);
+    y = (float)(x * sn + y * cs);
+    x = u;
+}
+
+// A workgroup takes the rows of one tile of positions, one KV head and up to two of
 // the query heads that share it (its first workgroup of them the keys and values
 // too).  The angle of a (position, pair) is computed once for all of these, in 64
 // bits: position * freq reaches 10^5 and more, and a key next to the border of two
 // codes must fall to the same side at every caller.  A thread has both values of its
 // pairs, so rows may be rotated in place; the keys go to the quantisation, which
-// takes whole blocks of 32, through LDS.
-template <int NB>
+// takes whole blocks of 32, through LDS.  WIDE: four pairs a thread, in 16-byte pieces
+// (dims a multiple of 8); else one.
+//
+// What bounds it: prompts of up to 1000 rows (2400 in all), 32 heads on 8 of 128, 96 dims
+// turning, rotated keys out as well: 109 MB, 21-23 us at a large copy's rate, take 26-28 in a kernel
+// trace; vector instructions (a third in 64 bits) issue in about a third of the cycles, the rest is
+// memory, the rows written among it at the launch's end (past the caches they take 37.4 us with
+// the read back, through them 39.7).  Four sequences of 8 rows 6.6: lengths, page, rows, angles one
+// after the other.  (One pair a thread 40 us; the pairs' layout not a template, 55 with the read back.)
+template <int NB, bool WIDE, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void kv4_append_rope_k(Kv4View c, holo_batch_t b, RopeRows a)
 {
-    constexpr int HD = 32 * NB, P = HD / 2, GROUPS = 256 / P, KS = HD + 4;
+    constexpr int HD = 32 * NB, N = WIDE ? 4 : 1, P = HD / (2 * N), GROUPS = 256 / P, KS = HD + 4;
+    typedef float vec __attribute__((ext_vector_type(N)));
     __shared__ __align__(16) float lk[32 * KS];
     __shared__ __align__(16) uint8_t lv[32 * HD];
     const Kv4Entry e = kv4_entry(c, b, blockIdx.z);
@@ -36,64 +64,93 @@ __global__ __launch_bounds__(256) void kv4_append_rope_k(Kv4View c, holo_batch_t
     const int from = e.len - e.rows;  // position of the entry's first row, which may be negative
     if ((int)blockIdx.x > (e.take + 30) / 32) return;
     const int t = (from >> 5) + (int)blockIdx.x, p0 = 32 * t;
-    const int lo = max(from - p0, 0), hi = min(from + e.take - p0, 32);
-    if (lo >= hi) return;
+    const int lo = max(from - p0, 0), hi = min(from + e.take - p0, 32), n = hi - lo;
+    if (n <= 0) return;
     const int64_t row0 = (int64_t)e.first + p0 - from;
     const bool keys = part == 0;
     uint8_t *tile = keys && t >= 0 ? kv4_tile<NB>(c, e, kvh, t) : nullptr;
 
     const int i = threadIdx.x % P, g = threadIdx.x / P;
-    const bool turns = 2 * i < a.r.dims;
-    // the pair's values: dims d0 and d1 of a head
-    const int d0 = turns && !a.r.interleaved ? i : 2 * i, d1 = turns && !a.r.interleaved ? i + a.r.dims / 2 : 2 * i + 1;
-    const double freq = turns ? a.r.freq[i] * M_1_PI : 0.0;
-    // groups of P threads take rows, and where there are few rows each some of the heads
-    const int n = hi - lo, slots = min(max(GROUPS / n, 1), max(heads + keys, 1)), rows = GROUPS / slots;
-    if (g < rows * slots)
-        for (int p = lo + g / slots; p < hi; p += rows) {
-            const int64_t row = row0 + p;
-            const float *qp = a.q + row * a.ldq + (int64_t)(kvh * G + h0) * HD;
-            float *qo = a.q_out + row * a.ldqo + (int64_t)(kvh * G + h0) * HD;
-            const float *kp = a.k + row * a.ldk + kvh * HD;
-            float x[kRopeHeads + 1], y[kRopeHeads + 1];
+    const bool turns = 2 * N * i < a.r.dims;
+    // the pairs' values: N of a head from d0 on, and N from d1 on
+    const int d0 = turns && !INTERLEAVED ? N * i : 2 * N * i, d1 = turns && !INTERLEAVED ? N * i + a.r.dims / 2 : 2 * N * i + N;
+    double freq[N], cs[N], sn[N];
 #pragma unroll
-            for (int j = 0; j <= kRopeHeads; j++) {  // head h0 + s; behind the last, the key
-                const int s = g % slots + j * slots;
-                if (s > heads || (s == heads && !keys)) break;
-                const float *at = s < heads ? qp + s * HD : kp;
-                x[j] = at[d0];
-                y[j] = at[d1];
-            }
-            double cs = 1.0, sn = 0.0;
-            if (turns) {
-                double turn = ((double)from + (double)(a.depth ? a.depth[row] : p + p0 - from)) * freq;  // half turns
-                turn -= 2.0 * rint(0.5 * turn);
-                sincospi(turn, &sn, &cs);
-                cs *= a.r.scale;
-                sn *= a.r.scale;
-            }
+    for (int k = 0; k < N; k++) freq[k] = turns ? a.r.freq[N * i + k] * M_1_PI : 0.0;
+    auto angles = [&](int p) {
+        if (!turns) return;
+        const double position = (double)from + (double)(a.depth ? a.depth[row0 + p] : p + p0 - from);
 #pragma unroll
-            for (int j = 0; j <= kRopeHeads; j++) {
-                const int s = g % slots + j * slots;
-                if (s > heads || (s == heads && !keys)) break;
-                float u = x[j], w = y[j];
-                if (turns) {
-                    u = (float)(x[j] * cs - y[j] * sn);
-                    w = (float)(x[j] * sn + y[j] * cs);
+        for (int k = 0; k < N; k++) turn_by(position, freq[k], a.r.scale, cs[k], sn[k]);
+    };
+    auto turn = [&](vec &x, vec &y) {
+        if (!turns) return;
+        float v[2 * N];
+#pragma unroll
+        for (int k = 0; k < N; k++) v[k] = x[k], v[N + k] = y[k];
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (INTERLEAVED && N > 1) turn_pair(v[2 * k], v[2 * k + 1], cs[k], sn[k]);
+            else turn_pair(v[k], v[N + k], cs[k], sn[k]);
+#pragma unroll
+        for (int k = 0; k < N; k++) x[k] = v[k], y[k] = v[N + k];
+    };
+    auto put_key = [&](int p, const vec &x, const vec &y) {
+        *(vec *)(lk + p * KS + d0) = x;
+        *(vec *)(lk + p * KS + d1) = y;
+        if (a.k_out) {
+            *(vec *)(a.k_out + (row0 + p) * a.ldko + kvh * HD + d0) = x;
+            *(vec *)(a.k_out + (row0 + p) * a.ldko + kvh * HD + d1) = y;
+        }
+    };
+    const float *q = a.q + (int64_t)(kvh * G + h0) * HD, *key = a.k + kvh * HD;
+    float *q_out = a.q_out + (int64_t)(kvh * G + h0) * HD;
+    if (g >= GROUPS) {
+    } else if (n >= GROUPS) {  // many rows: a group takes whole rows
+        for (int p = lo + g; p < hi; p += GROUPS) {
+            const float *in = q + (row0 + p) * a.ldq, *kin = key + (row0 + p) * a.ldk;
+            float *out = q_out + (row0 + p) * a.ldqo;
+            vec x[kRopeHeads], y[kRopeHeads], kx, ky;
+#pragma unroll
+            for (int j = 0; j < kRopeHeads; j++)
+                if (j < heads) {
+                    x[j] = *(const vec *)(in + j * HD + d0);
+                    y[j] = *(const vec *)(in + j * HD + d1);
                 }
-                if (s < heads) {
-                    qo[s * HD + d0] = u;
-                    qo[s * HD + d1] = w;
-                } else {
-                    lk[p * KS + d0] = u;
-                    lk[p * KS + d1] = w;
-                    if (a.k_out) {
-                        a.k_out[row * a.ldko + kvh * HD + d0] = u;
-                        a.k_out[row * a.ldko + kvh * HD + d1] = w;
-                    }
+            if (keys) {
+                kx = *(const vec *)(kin + d0);
+                ky = *(const vec *)(kin + d1);
+            }
+            angles(p);
+#pragma unroll
+            for (int j = 0; j < kRopeHeads; j++)
+                if (j < heads) {
+                    turn(x[j], y[j]);
+                    __builtin_nontemporal_store(x[j], (vec *)(out + j * HD + d0));
+                    __builtin_nontemporal_store(y[j], (vec *)(out + j * HD + d1));
                 }
+            if (keys) {
+                turn(kx, ky);
+                put_key(p, kx, ky);
             }
         }
+    } else {  // few: a head of a row
+        const int units = max(heads, 0) + keys;
+        for (int u = g; u < n * units; u += GROUPS) {
+            const int p = lo + u / units, s = u % units;
+            const float *in = s < heads ? q + (row0 + p) * a.ldq + s * HD : key + (row0 + p) * a.ldk;
+            vec x = *(const vec *)(in + d0), y = *(const vec *)(in + d1);
+            angles(p);
+            turn(x, y);
+            if (s < heads) {
+                float *out = q_out + (row0 + p) * a.ldqo + s * HD;
+                *(vec *)(out + d0) = x;
+                *(vec *)(out + d1) = y;
+            } else {
+                put_key(p, x, y);
+            }
+        }
+    }
     if (!tile) return;
     Kv4VWords<NB> words(tile, lo, hi);
     __syncthreads();
@@ -144,12 +201,17 @@ int holo_kv4_append_rope(const holo_kv4_t *c, int layer, const holo_rope_t *r, c
     const int take = b->max_rows < b->rows ? b->max_rows : b->rows;
     const dim3 grid((unsigned)(take + 30) / 32 + 1, (unsigned)(parts * c->n_kv_heads), b->n_seqs);
     const RopeRows a{*r, q, k, v, q_out, k_out, ldq, ldk, ldv, ldqo, ldko, n_heads, depth};
+    const bool wide = r->dims % 8 == 0;
     auto run = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream(), w, *b, a); };
+    auto pick = [&](auto nb) {
+        if (r->interleaved) wide ? run(kv4_append_rope_k<nb, true, true>) : run(kv4_append_rope_k<nb, false, true>);
+        else wide ? run(kv4_append_rope_k<nb, true, false>) : run(kv4_append_rope_k<nb, false, false>);
+    };
     switch (c->head_dim) {
-    case 32: run(kv4_append_rope_k<1>); break;
-    case 64: run(kv4_append_rope_k<2>); break;
-    case 96: run(kv4_append_rope_k<3>); break;
-    default: run(kv4_append_rope_k<4>); break;
+    case 32: pick(std::integral_constant<int, 1>()); break;
+    case 64: pick(std::integral_constant<int, 2>()); break;
+    case 96: pick(std::integral_constant<int, 3>()); break;
+    default: pick(std::integral_constant<int, 4>()); break;
     }
     HOLO_LAUNCH_CHECK();
     return 0;
