@@ -93,7 +93,7 @@ __device__ __forceinline__ Range draft_range(const Draft &d, int slot, int lane)
     const int l = __ffsll((unsigned long long)past) - 1;
     r.at = slot - __builtin_amdgcn_readlane(upto - n, l);
     r.entry = l * each;
-    for (;; r.entry++) {  // ends within the lane's entries: their ranges pass r.at
+    for (int i = 1; i < each; i++, r.entry++) {  // the lane's entries: their ranges pass r.at
         const int m = ranges_of(draft_tiles(d, r.entry), r.chunk);
         if (r.at < m) break;
         r.at -= m;
@@ -474,8 +474,9 @@ __global__ __launch_bounds__(256, CT == 1 && NB < 3 ? 3 : 2) void attn_draft_k(D
 {
     __shared__ __align__(16) DraftLds<NB, CT> lds;
     const Kv4Attn &a = d.a;
-    const int block = blockIdx.x / (8 * a.ctiles), in = blockIdx.x % (8 * a.ctiles), pair = 8 * block + (in & 7);
-    const int slot = pair / a.c.n_kv_heads, kvh = pair % a.c.n_kv_heads, ct = in >> 3;
+    const uint32_t id = blockIdx.x + blockIdx.y * gridDim.x;  // below 2^32 (run_draft)
+    const uint32_t in = id % (8u * a.ctiles), pair = id / (8u * a.ctiles) * 8 + (in & 7);
+    const int slot = (int)(pair / a.c.n_kv_heads), kvh = (int)(pair % a.c.n_kv_heads), ct = (int)(in >> 3);
     if (slot >= d.slots) return;
     Range r{slot, 0, 0x7FFFFFFF};
     if constexpr (CUT) r = draft_range(d, slot, threadIdx.x & 63);
@@ -503,7 +504,14 @@ static int run_draft(Draft d)
     const bool cuts = n <= 1024 && tiles * (d.cut - n * groups) > (int64_t)36 * d.cut;
     // (ranges: tiles / chunk of them and one more an entry at most)
     d.slots = (int)(cuts ? d.cut / groups + n : n);
-    const dim3 grid((unsigned)(((int64_t)d.slots * d.a.c.n_kv_heads + 7) / 8 * 8 * d.a.ctiles));
+    // (65535 entries by 65535 groups at most, rounded up to eight pairs; a row of the grid is whole eights)
+    const int64_t blocks = ((int64_t)d.slots * d.a.c.n_kv_heads + 7) / 8 * 8 * d.a.ctiles;
+    if (blocks > 0xFFF00000) {
+        HOLO_REJECT("holo_attention_kv4_draft: more rows and heads than one launch takes");
+        return HOLO_EINVAL;
+    }
+    const unsigned across = (unsigned)(blocks < 1 << 22 ? blocks : 1 << 22);
+    const dim3 grid(across, (unsigned)((blocks + across - 1) / across));
     if (!cuts) {
         hipLaunchKernelGGL((attn_draft_k<NB, CT, false>), grid, dim3(256), 0, stream(), d);
         HOLO_LAUNCH_CHECK();

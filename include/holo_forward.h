@@ -166,7 +166,8 @@ typedef struct {
  * holo_attention_packed; q_out the rotated queries.  q_out may be q and k_out k,
  * with the same ld; otherwise nothing that is written overlaps what is read.  A
  * row turns by len - r + i (row i of an entry of r rows), or with depth (device,
- * [rows]) by len - r + depth[row]: rows of a tree.  n_heads 0: no queries.
+ * [rows]) by len - r + depth[row]: rows of a tree.  n_heads 0: no queries; n_kv_heads
+ * times half the query heads of each (rounded up) up to 65535.
  * Rows without a page, or before position 0, are rotated all the same.  0 or
  * HOLO_EINVAL.  (cuda_rope_apply, cuda_ops.h:117, takes one row.)               */
 int holo_kv4_append_rope(const holo_kv4_t *c, int layer, const holo_rope_t *r, const float *q, const float *k,
@@ -220,7 +221,9 @@ int holo_draft_plan(const int *parent, int *depth, uint32_t *mask, int words, co
 /* holo_attention_kv4 of rows that see the positions before their entry's rows, and
  * of these the ones whose bits their mask has (any mask, its own row's bit too;
  * rows past the words have none).  A row that sees nothing gives zeros.  max_rows up
- * to 32 * words, words up to 32, otherwise as holo_attention_kv4.                 */
+ * to 32 * words, words up to 32, otherwise as holo_attention_kv4; n_seqs times the
+ * tiles of columns and KV heads up to some 4.29e9.  Ranges go by the lengths themselves, for
+ * up to 1024 entries: ragged batches, and long sequences beside short ones, need no calls of their own.  */
 int holo_attention_kv4_draft(const holo_kv4_t *c, int layer, float *out, const float *q, int ldo, int ldq,
                              int n_heads, const uint32_t *mask, int words, const holo_batch_t *b);
 

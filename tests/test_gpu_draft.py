@@ -428,6 +428,54 @@ def test_attention_is_not_touched_by_what_a_row_does_not_see(holo, heads, rows):
     assert np.isnan(got[:, g:, 32:]).all() and not np.isnan(got[~s[:, 1], g:, :32]).any()
 
 
+def test_attention_of_a_batch_of_many_entries(holo):
+    """More workgroups than one row of the grid has: 60000 entries by 80 tiles of columns, a few of them with rows."""
+    print("case draft attention 60000 entries", flush=True)
+    rng = np.random.default_rng(16)
+    hd, heads, n, lens = 32, 40, 60000, [40, 33, 3]
+    c = Cache(hd, 32, 1, heads, 6, 3, 2)
+    pages(c, lens, rng)
+    fill(c, rng, 0)
+    dev = OnDevice(holo, c)
+    rows, seqs = np.zeros(n, int), np.full(n, -1)
+    at = [7, 31234, n - 1]
+    rows[at], seqs[at] = [17, 32, 2], [0, 1, 2]
+    seen = [dm.seen_rows(dm.tree(rng, r, 2)) for r in (17, 32, 2)]
+    q = rng.standard_normal((51, heads * hd)).astype(np.float32)
+    got = attention(holo, dev, 0, q, rows.tolist(), heads, np.concatenate([dm.words(s, 1) for s in seen]), seqs=seqs)
+    assert normwise(got, dm.want_attention(c, 0, q, [17, 32, 2], [0, 1, 2], heads, seen)) <= TOL
+
+
+@pytest.mark.parametrize("n", [70, 300, 1024, 1025])
+def test_attention_of_many_ragged_sequences_in_ranges(holo, n):
+    """Ranges found from the lengths of more entries than a wave has lanes: entries without rows, empty sequences, one
+    sequence past max_len, and long ones between short ones."""
+    print(f"case draft attention ragged {n}", flush=True)
+    rng = np.random.default_rng(n)
+    hd, heads, n_kv = 32, 1, 1
+    lens = np.minimum(rng.integers(0, 60, n), 50)
+    long = rng.choice(n, 6, replace=False)
+    lens[long] = [1700, 900, 1311, 257, 1500, 2000]
+    c = Cache(hd, 64, 1, n_kv, int(sum(-(-x // 64) for x in lens)) + 1, n, 32)
+    pages(c, lens.tolist(), rng)
+    c.pool[:] = rng.integers(0, 256, c.pool.shape, dtype=np.uint8)
+    f = c.pool[..., 32 * hd:].view(np.uint16)  # scales of 0.5 to 2, either sign, in the cache's 8 significant bits
+    f[:] = (f & 0x83F8) | (0x3800 + (f & 0x0400))
+    dev = OnDevice(holo, c)
+    rows = rng.integers(0, 4, n)
+    rows[long] = 3
+    order = rng.permutation(n)
+    seen = [dm.seen_rows(dm.tree(rng, int(r), 2)) for r in rows[order]]
+    mask = np.concatenate([dm.words(s, 1) for s in seen if len(s)])
+    q = rng.standard_normal((int(rows.sum()), heads * hd)).astype(np.float32)
+    got = attention(holo, dev, 0, q, rows[order].tolist(), heads, mask, seqs=order, max_len=1700)
+    want = dm.want_attention(c, 0, q, rows[order].tolist(), order.tolist(), heads, seen)
+    first = np.cumsum([0, *rows[order]])[list(order).index(long[5])]
+    assert np.isnan(got[first:first + 3]).all()  # 2000 positions
+    keep = np.delete(np.arange(len(q)), range(first, first + 3))
+    assert normwise(got[keep], want[keep]) <= TOL
+
+
 # ---- softmax ---------------------------------------------------------------------------------------------
 
 def softmax(holo, x, scale, ldx=None, ldd=None, in_place=False, shift=0):
@@ -667,6 +715,34 @@ def test_verification_of_rows_out_of_place(holo):
             assert path[:3].tolist() == want + [-1] * (3 - len(want)) and after[0] == token and (path[3:7] == -7).all()
             want, token, _ = dm.verify([-1, 0, 1], tokens[7:], np.float32(u[7:]), p, p, mode)
             assert path[7:10].tolist() == want + [-1] * (3 - len(want)) and after[1] == token and (path[10:] == -7).all()
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_verification_of_many_entries_keeps_the_targets_distribution(holo, mode):
+    """60000 entries of the same distributions: the first token behind row 0 has the target's probabilities, within five
+    standard deviations of a share; every entry as the model has it."""
+    print(f"case verify law {mode}", flush=True)
+    rng = np.random.default_rng(17)
+    n, t = 60000, [-1, 0, 0, 1]
+    p = np.float32([0.4, 0.3, 0.15, 0.1, 0.05, 0])
+    q = np.float32([0.1, 0.2, 0.2, 0.25, 0.15, 0.1])
+    tokens = rng.integers(0, 6, (n, 4))
+    for i in range(n if mode != "chosen" else 0):
+        tokens[i, 1:3] = rng.choice(6, 2, mode == "drawn", q.astype(np.float64) / q.sum(dtype=np.float64))
+    if mode == "chosen":
+        tokens[:, 1:3] = (3, 1)
+    u = rng.random((n, 4)).astype(np.float32)
+    path, n_path, after = verify(holo, [4] * n, [t] * n, tokens.ravel(), u.ravel(), np.tile(p, (4 * n, 1)),
+                                 np.tile(q, (4 * n, 1)), mode)
+    path = path.reshape(n, 4)
+    first = np.where(n_path > 1, tokens[np.arange(n), path[:, 1]], after)
+    share = np.bincount(first, minlength=6) / n
+    assert (np.abs(share - p) <= 5 * np.sqrt(p * (1 - p) / n) + 1e-7).all()
+    for i in range(0, n, 29):
+        want, token, margin = dm.verify(t, tokens[i], u[i], np.tile(p, (4, 1)), np.tile(q, (4, 1)), mode)
+        # (0.1 * 3 and the like lie on the borders of sums of 0.3: those are for either side)
+        if margin > 1e-12:
+            assert path[i].tolist() == want + [-1] * (4 - len(want)) and after[i] == token
 
 
 # ---- the rows that stand ------------------------------------------------------------------------------------
