@@ -949,3 +949,91 @@ def test_steps_of_drafted_rows(holo, hd, heads, n_kv, page_len, captured):
         lib.holo_set_stream(before)
         lib.holo_stream_destroy(st)
         lib.holo_kv4_pages_destroy(handle)
+
+
+@pytest.mark.parametrize("hd,heads,rows,vocab", [(64, 4, 5, 3000), (128, 32, 20, 40000)])
+def test_two_graphs_at_once(holo, hd, heads, rows, vocab):
+    """Attention in ranges and verification, captured on two streams and replayed together, after lengths, masks, random
+    numbers and probabilities changed; eager calls between the replays.  The second size's partial sums are past 1 MiB."""
+    print(f"case draft two graphs hd {hd} rows {rows}", flush=True)
+    rng = np.random.default_rng(hd)
+    lib, n_kv, n = holo.lib(), max(heads // 4, 1), 2500 if hd == 64 else 1700
+    before, streams, sides = lib.holo_get_stream(), [lib.holo_stream_create() for _ in range(2)], []
+    dim = heads * hd
+    new = holo.DeviceBuffer
+    try:
+        for side in range(2):
+            c = Cache(hd, 64, 1, n_kv, 60, 2, 50)
+            pages(c, [n + 6, 100], rng)
+            c.len[:] = (n, 90)
+            c.pool[:] = rng.integers(0, 256, c.pool.shape, dtype=np.uint8)
+            f = c.pool[..., 32 * hd:].view(np.uint16)  # scales of 1/16 to 1/4, in the cache's 8 significant bits
+            f[:] = (f & 0x83F8) | (0x2C00 + (f & 0x0400))
+            dev, b = OnDevice(holo, c), Batch(holo, [rows, 3], [0, 1], None, 3000)
+            total = rows + 3
+            d = dict(q=new(4 * total * dim), o=new(4 * total * dim), mask=new(4 * total), parent=new(4 * total),
+                     depth=new(4 * total), p=new(4 * total * vocab), d=new(4 * total * vocab), tokens=new(4 * total),
+                     u=new(4 * total), path=new(4 * total), count=new(8), next=new(8))
+
+            def issue(dev=dev, b=b, d=d):
+                assert lib.holo_draft_plan(d["parent"].ptr, d["depth"].ptr, d["mask"].ptr, 1, b.ref) == 0
+                assert lib.holo_attention_kv4_draft(dev.ref, 0, d["o"].ptr, d["q"].ptr, dim, dim, heads, d["mask"].ptr, 1,
+                                                    b.ref) == 0
+                assert lib.holo_draft_verify(d["path"].ptr, d["count"].ptr, d["next"].ptr, d["p"].ptr, d["d"].ptr, vocab,
+                                             vocab, vocab, d["tokens"].ptr, d["parent"].ptr, d["u"].ptr,
+                                             holo.DRAFT_DISTINCT, b.ref) == 0
+
+            lib.holo_set_stream(streams[side])
+            assert lib.holo_graph_begin() == 0
+            issue()
+            graph = lib.holo_graph_end()
+            assert graph
+            holo.check("capture")
+            sides.append((c, dev, b, d, issue, graph))
+        for step in range(3):
+            wants = []
+            for side, (c, dev, b, d, issue, graph) in enumerate(sides):
+                lib.holo_set_stream(streams[side])
+                c.len += 1
+                dev.refresh()
+                parents = [dm.tree(rng, k, 3) for k in (rows, 3)]
+                seen = [dm.seen_rows(t) for t in parents]
+                total = rows + 3
+                q = rng.standard_normal((total, dim)).astype(np.float32)
+                z = (2 * rng.standard_normal((total, vocab))).astype(np.float32)
+                p, r = np.exp(z), np.exp(z + rng.standard_normal(z.shape).astype(np.float32))
+                p, r = (x / x.sum(1, keepdims=True) for x in (p, r))
+                flat = [x for t in parents for x in t]
+                first = [0] * rows + [rows] * 3
+                tokens = np.int32([r[first[i] + max(x, 0)].argsort()[-1 - i % 3] for i, x in enumerate(flat)])
+                u = rng.random(total).astype(np.float32)
+                for name, x in (("q", q), ("parent", np.int32(flat)), ("p", p), ("d", r), ("tokens", tokens), ("u", u)):
+                    d[name].upload(np.ascontiguousarray(x))
+                paths = [dm.verify(parents[i], tokens[a:e], u[a:e], p[a:e], r[a:e], "distinct")
+                         for i, (a, e) in enumerate(((0, rows), (rows, total)))]
+                wants.append((dm.want_attention(c, 0, q, [rows, 3], [0, 1], heads, seen), paths))
+            lib.cuda_sync()
+            for side in range(2):  # both under way at once
+                lib.holo_set_stream(streams[side])
+                assert lib.holo_graph_launch(sides[side][5]) == 0
+            for again in range(2):  # then the same calls eagerly
+                lib.cuda_sync()
+                holo.check("replay")
+                for side, ((c, dev, b, d, issue, graph), (want, paths)) in enumerate(zip(sides, wants)):
+                    assert normwise(d["o"].download(np.float32).reshape(want.shape), want) <= TOL
+                    path, count, after = (d[x].download(np.int32) for x in ("path", "count", "next"))
+                    for i, (rows_of, token, margin) in enumerate(paths):
+                        a, e = ((0, rows), (rows, rows + 3))[i]
+                        assert margin > 1e-12
+                        assert path[a:e].tolist() == rows_of + [-1] * (e - a - len(rows_of))
+                        assert count[i] == len(rows_of) and after[i] == token
+                    if not again:
+                        d["o"].upload(np.zeros(want.shape, np.float32))
+                        lib.holo_set_stream(streams[side])
+                        issue()
+    finally:
+        for *_, graph in sides:
+            lib.holo_graph_destroy(graph)
+        lib.holo_set_stream(before)
+        for s in streams:
+            lib.holo_stream_destroy(s)
