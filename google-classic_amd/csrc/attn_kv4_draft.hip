@@ -12,11 +12,11 @@
 //
 // What bounds it (32 heads on 8 of 128): 63 rows over 100063 positions take 222-227 us, 465
 // TFLOP/s of scores and values, twice that on the matrix cores for the halves: 0.93 of the
-// 1.14 PFLOP/s of a large f16 product, which is where the matrix cores are throttled (busy in
-// 47% of the cycles at most); matrix and vector instructions of a SIMD's two waves hardly
-// overlap (2640 cycles a tile and 32 columns, of which they issue in 1024 and 1376).  64 x 5 rows of up to
-// 8192 140-146 us, 3.2 TB/s, 20 of 32 columns in use; 16 x 26 of up to 4096 53; 5 rows of
-// 517 positions 9.0, a chain of five tiles of 1.05 each and the launch.
+// 1.14 PFLOP/s that a large f16 product reaches here.  Matrix and vector instructions of a
+// SIMD's two waves hardly overlap: they issue in 40% and 53% of the cycles.  64 x 5 rows of up to
+// 8192 140-146 us, 3.2 TB/s, 20 of 32 columns in use, 33% and 44%; 16 x 26 of up to 4096 53, the
+// longest sequences' workgroups (mean 67 tiles, the longest 128); 5 rows of 517 positions 9.0,
+// a chain of five tiles of 1.05 each and the launch.
 //
 // Tried: the tiles unpacked once into LDS for 64 or 128 columns of four waves, a tile
 // ahead, with the keys a tile before the values and with matrix and vector instructions
