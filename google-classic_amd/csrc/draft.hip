@@ -373,21 +373,22 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_k(Verify a, holo_
         }
     } else {
         // nothing weighs: the target's most probable token, the lowest of equals
-        float best = -FLT_MAX;
-        for (int t = lane; t < a.vocab; t += 64)
-            if (p[t] > best || (token < 0 && p[t] == p[t])) {
-                best = p[t];
-                token = t;
-            }
-        for (int off = 32; off > 0; off >>= 1) {
-            const float v = __shfl_xor(best, off, 64);
-            const int t = __shfl_xor(token, off, 64);
-            if (t >= 0 && (token < 0 || v > best || (v == best && t < token))) {
+        float best = -1.f;
+        for (int t = lane; t < a.vocab; t += 64) {
+            const float v = probability(p[t]);
+            if (v > best) {
                 best = v;
                 token = t;
             }
         }
-        token = max(token, 0);
+        for (int off = 32; off > 0; off >>= 1) {
+            const float v = __shfl_xor(best, off, 64);
+            const int t = __shfl_xor(token, off, 64);
+            if (v > best || (v == best && t < token)) {
+                best = v;
+                token = t;
+            }
+        }
     }
     if (lane == 0) {
         a.n_path[blockIdx.x] = w.s.count;

@@ -118,7 +118,7 @@ def verify(parent, tokens, u, target, draft, mode):
             w[x] = 0.0
     sums = np.cumsum(w)
     if sums[-1] == 0:
-        return path, int(np.nanargmax(target[node])), margin
+        return path, int(probability(target[node]).argmax()), margin
     at = float(u[0]) * sums[-1]
     x = int(np.searchsorted(sums, at, side="right"))
     margin = min(margin, np.abs(sums[w > 0] - at).min() / sums[-1])
