@@ -137,92 +137,105 @@ __global__ __launch_bounds__(256) void kv4_read_k(Kv4View c, holo_batch_t b, flo
 // group), the VW dims of eight positions' values.
 //
 // What bounds it: one sequence, 32 layers of 8 heads, four rows moved 5.2-5.5 us, a chain of
-// lengths, path, pages and words, and code that a CU has not run yet.  64 sequences 28 us: 16384
-// workgroups, four to a place on the chip, each that chain; the bytes (28 MB read, 28
-// written: pieces of 64, where the rows themselves are 9.4 and 9.4) would take 11.  Two heads
-// a workgroup 30.5 and 7.5, four 42 and 11.7; loads without branches 31-37.
+// lengths, path, pages and words, and code that a CU has not run yet.  64 sequences 24-25 us (20
+// in a trace): 16384 workgroups of a wave, two to a place on the chip, each that chain; the
+// bytes (28 MB read, 28 written: pieces of 64, where the rows themselves are 9.4 and 9.4)
+// would take 11.  With a tile's halves in two waves 28 (27 in a trace; one sequence the same);
+// of those, two heads a workgroup 30.5 and 7.5, four 42 and 11.7, loads without branches 31-37.
 template <int NB>
-__global__ __launch_bounds__(NB == 3 ? 192 : 128) void kv4_keep_k(Kv4View c, holo_batch_t b, const int *path,
-                                                                 const int *n_path)
+__global__ __launch_bounds__(64) void kv4_keep_k(Kv4View c, holo_batch_t b, const int *path, const int *n_path)
 {
-    constexpr int HD = 32 * NB, T = NB == 3 ? 192 : 128, VW = VWords<NB>::W, M = 2 * NB;
+    constexpr int HD = 32 * NB, VW = VWords<NB>::W, CH = 2 * NB / VW, SC = (NB + 1) / 2;
     __shared__ const uint8_t *src[32];  // the tile that a position's row comes from; nullptr: it stays
     __shared__ int at[32];              // and the place there
-    __shared__ int some;
     const int s = blockIdx.z, kvh = blockIdx.x;
     c.layer_tiles *= blockIdx.y;
     const Kv4Entry e = kv4_entry(c, b, s);
     const int n = min(n_path[s], e.take), from = e.len - e.rows;
     const int end = min(from + max(n, 0), e.len);  // positions written: up to here
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x, r = lane & 15, g = lane >> 4;
     for (int t = max(from, 0) >> 5; 32 * (int64_t)t < end; t++) {
         uint8_t *tile = kv4_tile<NB>(c, e, kvh, t);
-        if (threadIdx.x < 64) {
-            const uint8_t *of = nullptr;
-            const int i = 32 * t + (int)threadIdx.x - from;
-            if (tile && threadIdx.x < 32 && i >= 0 && i < n) {
-                const int p = path[e.first + i];
-                if (p != i && p >= 0 && p < e.rows && from + p >= 0) {
-                    of = kv4_tile<NB>(c, e, kvh, (from + p) >> 5);
-                    at[threadIdx.x] = (from + p) & 31;
-                }
+        const uint8_t *of = nullptr;
+        const int i = 32 * t + lane - from;
+        if (tile && lane < 32 && i >= 0 && i < n) {
+            const int p = path[e.first + i];
+            if (p != i && p >= 0 && p < e.rows && from + p >= 0) {
+                of = kv4_tile<NB>(c, e, kvh, (from + p) >> 5);
+                at[lane] = (from + p) & 31;
             }
-            if (threadIdx.x < 32) src[threadIdx.x] = of;
-            const bool any = __any(of != nullptr);
-            if (threadIdx.x == 0) some = any;
+        }
+        if (!__any(of != nullptr)) continue;
+        if (lane < 32) src[lane] = of;
+        __syncthreads();
+        // keys of position 16 half + r, lane group g
+        uint32_t kw[2][NB];
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint8_t *f = src[16 * half + r];
+            if (!f) continue;
+            const int sp = at[16 * half + r];
+            const uint32_t *w = (const uint32_t *)f + NB * (64 * (sp >> 4) + 16 * g + (sp & 15));
+#pragma unroll
+            for (int j = 0; j < NB; j++) kw[half][j] = w[j];
+        }
+        // values of dims 16 m + r, m = VW chunk .., at eight positions
+        uint32_t *vw = (uint32_t *)(tile + 16 * HD);
+        uint32_t put[CH][VW] = {}, mask = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint8_t *f = src[v_pos(g, j)];
+            if (!f) continue;
+            const int sp = at[v_pos(g, j)], slot = 4 * (sp >> 4) + (sp & 3);
+            const uint32_t *w = (const uint32_t *)(f + 16 * HD) + VW * (16 * ((sp & 15) >> 2) + r);
+            uint32_t x[CH][VW];
+#pragma unroll
+            for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+                for (int i = 0; i < VW; i++) x[ch][i] = w[64 * VW * ch + i];
+            mask |= 15u << word_shift(j);
+#pragma unroll
+            for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+                for (int i = 0; i < VW; i++) put[ch][i] |= (x[ch][i] >> word_shift(slot) & 15u) << word_shift(j);
+        }
+        if (mask)
+#pragma unroll
+            for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+                for (int i = 0; i < VW; i++) put[ch][i] |= vw[VW * (64 * ch + lane) + i] & ~mask;
+        // scales of (position, block)
+        const int pos = lane & 31;
+        const uint8_t *ss = src[pos];
+        uint16_t kd[SC], vd[SC];
+        if (ss) {
+            const int p = at[pos];
+#pragma unroll
+            for (int k = 0; k < SC; k++) {
+                const int blk = min(2 * k + (lane >> 5), NB - 1);
+                kd[k] = ((const uint16_t *)(ss + 32 * HD))[32 * blk + 2 * (p & 15) + (p >> 4)];
+                vd[k] = ((const uint16_t *)(ss + 34 * HD))[32 * blk + 8 * ((p & 15) >> 2) + 4 * (p >> 4) + (p & 3)];
+            }
         }
         __syncthreads();
-        if (some) {
-            // keys of position 16 half + r, dims 8 (NB g ..)
-            const int half = threadIdx.x >> 6, kpos = 16 * half + r;
-            uint32_t kw[NB];
-            const uint8_t *ks = half < 2 ? src[kpos & 31] : nullptr;
-            if (ks) {
-                const uint32_t *w = (const uint32_t *)ks + NB * (64 * (at[kpos] >> 4) + 16 * g + (at[kpos] & 15));
 #pragma unroll
-                for (int j = 0; j < NB; j++) kw[j] = w[j];
+        for (int half = 0; half < 2; half++)
+            if (src[16 * half + r])
+#pragma unroll
+                for (int j = 0; j < NB; j++) ((uint32_t *)tile)[NB * (64 * half + lane) + j] = kw[half][j];
+        if (mask)
+#pragma unroll
+            for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+                for (int i = 0; i < VW; i++) vw[VW * (64 * ch + lane) + i] = put[ch][i];
+        if (ss)
+#pragma unroll
+            for (int k = 0; k < SC; k++) {
+                const int blk = 2 * k + (lane >> 5);
+                if (blk >= NB) continue;
+                ((uint16_t *)(tile + 32 * HD))[32 * blk + 2 * (pos & 15) + (pos >> 4)] = kd[k];
+                ((uint16_t *)(tile + 34 * HD))[32 * blk + 8 * ((pos & 15) >> 2) + 4 * (pos >> 4) + (pos & 3)] = vd[k];
             }
-            // values of dims 16 m + r, m = VW chunk .., at eight positions
-            const int chunk = threadIdx.x >> 6;
-            uint32_t *vw = (uint32_t *)(tile + 16 * HD) + VW * threadIdx.x;
-            uint32_t old[VW], put[VW] = {}, mask = 0;
-            if (VW * chunk < M) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int p = v_pos(g, j);
-                    if (!src[p]) continue;
-                    const int sp = at[p], slot = 4 * (sp >> 4) + (sp & 3);
-                    const uint32_t *w = (const uint32_t *)(src[p] + 16 * HD) +
-                                        VW * (64 * chunk + 16 * ((sp & 15) >> 2) + r);
-                    mask |= 15u << word_shift(j);
-#pragma unroll
-                    for (int i = 0; i < VW; i++) put[i] |= (w[i] >> word_shift(slot) & 15u) << word_shift(j);
-                }
-                if (mask)
-#pragma unroll
-                    for (int i = 0; i < VW; i++) old[i] = vw[i];
-            }
-            // scales of (position, block)
-            const int sp = threadIdx.x & 31, blk = threadIdx.x >> 5;
-            uint16_t kd = 0, vd = 0;
-            const uint8_t *ss = blk < NB ? src[sp] : nullptr;
-            if (ss) {
-                const int p = at[sp];
-                kd = ((const uint16_t *)(ss + 32 * HD))[32 * blk + 2 * (p & 15) + (p >> 4)];
-                vd = ((const uint16_t *)(ss + 34 * HD))[32 * blk + 8 * ((p & 15) >> 2) + 4 * (p >> 4) + (p & 3)];
-            }
-            __syncthreads();
-            if (ks)
-#pragma unroll
-                for (int j = 0; j < NB; j++) ((uint32_t *)tile)[NB * (64 * half + lane) + j] = kw[j];
-            if (mask)
-#pragma unroll
-                for (int i = 0; i < VW; i++) vw[i] = (old[i] & ~mask) | put[i];
-            if (ss) {
-                ((uint16_t *)(tile + 32 * HD))[32 * blk + 2 * (sp & 15) + (sp >> 4)] = kd;
-                ((uint16_t *)(tile + 34 * HD))[32 * blk + 8 * ((sp & 15) >> 2) + 4 * (sp >> 4) + (sp & 3)] = vd;
-            }
-        }
         __syncthreads();
     }
 }
@@ -468,10 +481,10 @@ int holo_kv4_keep(const holo_kv4_t *c, const int *path, const int *n_path, const
     const Kv4View w = kv4_view(c, 1);  // (the kernel takes layer_tiles times its layer)
     const dim3 grid(c->n_kv_heads, c->n_layers, b->n_seqs);
     switch (c->head_dim) {
-    case 32: hipLaunchKernelGGL(kv4_keep_k<1>, grid, dim3(128), 0, stream(), w, *b, path, n_path); break;
-    case 64: hipLaunchKernelGGL(kv4_keep_k<2>, grid, dim3(128), 0, stream(), w, *b, path, n_path); break;
-    case 96: hipLaunchKernelGGL(kv4_keep_k<3>, grid, dim3(192), 0, stream(), w, *b, path, n_path); break;
-    default: hipLaunchKernelGGL(kv4_keep_k<4>, grid, dim3(128), 0, stream(), w, *b, path, n_path); break;
+    case 32: hipLaunchKernelGGL(kv4_keep_k<1>, grid, dim3(64), 0, stream(), w, *b, path, n_path); break;
+    case 64: hipLaunchKernelGGL(kv4_keep_k<2>, grid, dim3(64), 0, stream(), w, *b, path, n_path); break;
+    case 96: hipLaunchKernelGGL(kv4_keep_k<3>, grid, dim3(64), 0, stream(), w, *b, path, n_path); break;
+    default: hipLaunchKernelGGL(kv4_keep_k<4>, grid, dim3(64), 0, stream(), w, *b, path, n_path); break;
     }
     HOLO_LAUNCH_CHECK();
     return 0;
