@@ -142,6 +142,7 @@ __global__ __launch_bounds__(256) void kv4_read_k(Kv4View c, holo_batch_t b, flo
 // bytes (28 MB read, 28 written: pieces of 64, where the rows themselves are 9.4 and 9.4)
 // would take 11.  With a tile's halves in two waves 28 (27 in a trace; one sequence the same);
 // of those, two heads a workgroup 30.5 and 7.5, four 42 and 11.7, loads without branches 31-37.
+// Four heads in four waves of a workgroup: 20 in a trace as well, one sequence 6.3 for 5.9.
 template <int NB>
 __global__ __launch_bounds__(64) void kv4_keep_k(Kv4View c, holo_batch_t b, const int *path, const int *n_path)
 {

@@ -797,6 +797,92 @@ def test_kept_rows_within_bounds(holo):
     assert np.array_equal(dev.bytes(), c.pool)
 
 
+# ---- offsets that 32 bits do not hold -------------------------------------------------------------------------
+
+def attend_held(q, hk, hv, heads, hd, seen):
+    """Attention of q's rows over values [n][n_kv * hd]; seen [rows][n]."""
+    out, group = np.zeros((len(q), heads, hd)), heads * hd // hk.shape[1]
+    for i in range(len(q)):
+        for h in range(heads):
+            x = slice(h // group * hd, (h // group + 1) * hd)
+            out[i, h] = attend(q[i, h * hd:(h + 1) * hd], hk[:, x], hv[:, x], seen[i])
+    return out.reshape(len(q), -1)
+
+
+def test_a_pool_past_four_gigabytes(holo):
+    """Pages whose bytes lie past 2^32: rows rotated into them, a tree's attention, the rows that stand."""
+    print("case draft large pool", flush=True)
+    rng = np.random.default_rng(21)
+    hd, heads, n_kv, n, rows, layer = 128, 8, 8, 1500, 26, 7
+    c = Cache(hd, 1024, 1, n_kv, 1, 1, 2)  # the arrays around a pool that only the device holds
+    dev, lib = OnDevice(holo, c), holo.lib()
+    dev.desc.n_layers, dev.desc.n_pages = 8, 500
+    size = lib.holo_kv4_page_bytes(dev.ref)
+    assert 470 * size > 1 << 32
+    dev.pool = holo.DeviceBuffer(500 * size)
+    dev.desc.pool = dev.pool.ptr
+    c.table[0], c.len[0] = (499, 470), n
+    dev.refresh()
+    dim = n_kv * hd
+    k, v = rng.standard_normal((2, n, dim)).astype(np.float32)
+    q = rng.standard_normal((n, heads * hd)).astype(np.float32)
+    dk, dv, dq, do = up(holo, k), up(holo, v), up(holo, q), holo.DeviceBuffer(q.nbytes)
+    df = up(holo, np.zeros(hd // 2))  # no angle: rows as they are
+    rope = holo.Rope(freq=df.ptr, dims=hd, interleaved=0, scale=1.0)
+    b, last = Batch(holo, [n], None, None, n), Batch(holo, [rows], None, None, n)
+    parent = dm.tree(rng, rows, 3)
+    seen = dm.seen_rows(parent)
+    mask, path, n_path = up(holo, dm.words(seen, 1)), up(holo, np.int32([0, 3, 4, 11, 25] + [-1] * 21)), up(holo, np.int32([5]))
+    for i in range(8):  # (every layer: the rows that stand are moved in all of them)
+        assert lib.holo_kv4_append_rope(dev.ref, i, C.byref(rope), dq.ptr, dk.ptr, dv.ptr, dim, dim, dim, dq.ptr, None, dim, 0,
+                                        heads, None, b.ref) == 0
+    assert lib.holo_attention_kv4_draft(dev.ref, layer, do.ptr, dq.ptr + 4 * (n - rows) * dim, dim, dim, heads, mask.ptr, 1,
+                                        last.ref) == 0
+    lib.cuda_sync()
+    holo.check("large pool")
+    assert np.array_equal(dq.download(np.float32), q.ravel())
+    hk, hv = values(*quantise(k)), values(*quantise(v))
+    see = np.concatenate([np.ones((rows, n - rows), bool), seen], 1)
+    got = do.download(np.float32)[:rows * dim].reshape(rows, dim)
+    assert normwise(got, attend_held(q[n - rows:], hk, hv, heads, hd, see)) <= TOL
+    assert lib.holo_kv4_keep(dev.ref, path.ptr, n_path.ptr, last.ref) == 0
+    for x in (hk, hv):
+        x[n - rows:n - rows + 5] = x[n - rows + np.array([0, 3, 4, 11, 25])]
+    for i in (0, layer):
+        assert lib.holo_kv4_read(dev.ref, i, dk.ptr, dv.ptr, dim, dim, b.ref) == 0
+        lib.cuda_sync()
+        holo.check("large pool, kept")
+        assert np.array_equal(dk.download(np.float32), hk.ravel()) and np.array_equal(dv.download(np.float32), hv.ravel())
+
+
+def test_the_last_positions_there_are(holo):
+    """A sequence of 0x7FFFF000 positions, of which the last page is there: a tree's attention, the rows that stand."""
+    print("case draft last positions", flush=True)
+    rng = np.random.default_rng(22)
+    hd, rows, n, held = 32, 20, 0x7FFFF000, 1024
+    c = Cache(hd, 1024, 1, 1, 2, 1, n // 1024)
+    c.table[0, -1], c.len[0] = 1, n
+    dev, lib = OnDevice(holo, c), holo.lib()
+    k, v, q = rng.standard_normal((3, held, hd)).astype(np.float32)
+    dk, dv, dq, do = up(holo, k), up(holo, v), up(holo, q), holo.DeviceBuffer(4 * rows * hd)
+    held_rows = Batch(holo, [held], None, None, n)
+    assert lib.holo_kv4_append(dev.ref, 0, dk.ptr, dv.ptr, hd, hd, held_rows.ref) == 0
+    hk, hv = values(*quantise(k)), values(*quantise(v))
+    seen = dm.seen_rows(dm.tree(rng, rows, 2))
+    see = np.concatenate([np.ones((rows, held - rows), bool), seen], 1)
+    mask, b = up(holo, dm.words(seen, 1)), Batch(holo, [rows], None, None, n)
+    path, n_path = up(holo, np.int32([0, 2, 3, 19] + [-1] * 16)), up(holo, np.int32([4]))
+    assert lib.holo_attention_kv4_draft(dev.ref, 0, do.ptr, dq.ptr, hd, hd, 1, mask.ptr, 1, b.ref) == 0
+    assert lib.holo_kv4_keep(dev.ref, path.ptr, n_path.ptr, b.ref) == 0
+    assert lib.holo_kv4_read(dev.ref, 0, dk.ptr, dv.ptr, hd, hd, held_rows.ref) == 0
+    lib.cuda_sync()
+    holo.check("last positions")
+    assert normwise(do.download(np.float32).reshape(rows, hd), attend_held(q[:rows], hk, hv, 1, hd, see)) <= TOL
+    for x, got in ((hk, dk), (hv, dv)):
+        x[held - rows:held - rows + 4] = x[held - rows + np.array([0, 2, 3, 19])]
+        assert np.array_equal(got.download(np.float32), x.ravel())
+
+
 # ---- all of it ---------------------------------------------------------------------------------------------------
 
 class Step:
