@@ -10,7 +10,7 @@
 // for both.  Sequences are cut into ranges of one length (not as many for each), so that a
 // batch's long and short ones end together.
 //
-// What bounds it (32 heads on 8 of 128): 63 rows over 100063 positions take 222-227 us, 465
+// What bounds it (32 heads on 8 of 128): 63 rows over 100063 positions take 222-228 us, 465
 // TFLOP/s of scores and values, twice that on the matrix cores for the halves: 0.93 of the
 // 1.14 PFLOP/s that a large f16 product reaches here.  Matrix and vector instructions of a
 // SIMD's two waves hardly overlap: they issue in 40% and 53% of the cycles.  64 x 5 rows of up to
