@@ -101,12 +101,15 @@ __device__ __forceinline__ double wave_scan(double v, int lane)
 // +normal values pass).
 __device__ __forceinline__ float probability(float p) { return __builtin_amdgcn_classf(p, 0x180) ? p : 0.f; }
 
-// max(p - beta q, 0)
+// max(p - beta q, 0), of one rounding: every place that asks for a token's weight gets the same.
 __device__ __forceinline__ double weight(float p, float q, double beta)
 {
-    const double w = (double)probability(p) - beta * (double)probability(q);
+    const double w = fma(-beta, (double)probability(q), (double)probability(p));
     return w > 0.0 ? w : 0.0;
 }
+
+// A random number: what lies outside [0, 1) is the nearest number inside, NaN is 0.
+__device__ __forceinline__ float unit(float u) { return fminf(fmaxf(u, 0.f), 0x1.fffffep-1f); }
 
 // Where a walk stands (the formulas: holo_forward.h).
 struct WalkState {
@@ -139,7 +142,7 @@ struct Walk {
         p = q = 0.f;
         if (up < 0) return;
         tok = a.tokens[first + i];
-        u = a.u[first + i];
+        u = unit(a.u[first + i]);
         if (tok < 0 || tok >= a.vocab) {
             tok = -1;
             return;
@@ -276,11 +279,11 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_k(Verify a, holo_
     const bool drawn = a.mode != HOLO_DRAFT_CHOSEN;
     const int nsums = (a.vocab + a.block - 1) / a.block, per = (nsums + 63) / 64;
     for (int i = threadIdx.x; i < nsums; i += kVerifyThreads) sums[i] = a.sums[(int64_t)blockIdx.x * nsums + i];
-    // Sum of all blocks; upto: of those up to the end of this lane's.
-    auto total = [&](double &upto) {
-        double s = 0.0;
-        for (int i = lane * per; i < min((lane + 1) * per, nsums); i++) s += sums[i];
-        upto = wave_scan(s, lane);
+    // Sum of all blocks; own: of this lane's, upto: of those up to the end of this lane's.
+    auto total = [&](double &own, double &upto) {
+        own = 0.0;
+        for (int i = lane * per; i < min((lane + 1) * per, nsums); i++) own += sums[i];
+        upto = wave_scan(own, lane);
         return __shfl(upto, 63, 64);
     };
 
@@ -296,8 +299,8 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_k(Verify a, holo_
         const int node = w.s.node;
         const double beta = w.s.beta;
         if (wave == 0) {
-            double upto;
-            w.s.left = total(upto);
+            double own, upto;
+            w.s.left = total(own, upto);
             w.go([&](int i, int row) {
                 if (lane == 0) a.path[first + i] = row;
             });
@@ -346,13 +349,14 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_k(Verify a, holo_
     __syncthreads();
     if (wave != 0) return;
     for (int i = w.s.count + lane; i < take; i += 64) a.path[first + i] = -1;
-    double upto;
-    const double all = total(upto), at = (double)a.u[first] * all;
+    double own, upto;
+    const double all = total(own, upto), at = (double)unit(a.u[first]) * all;
     int token = -1;
     if (all > 0.0) {
-        // the first lane, block and token whose sum passes; past them by rounding: the last with a weight
-        const double mine = upto - __shfl_up(upto, 1, 64);
-        const uint64_t some = __ballot(lane == 0 ? upto > 0.0 : mine > 0.0), pass = __ballot(upto > at) & some;
+        // The first lane, block and token whose sum passes; past them by rounding: the last with
+        // a weight.  Only lanes whose own blocks weigh count: the scan adds in another order in
+        // every lane, and one without any weight can have a sum a rounding above its neighbour's.
+        const uint64_t some = __ballot(own > 0.0), pass = __ballot(upto > at) & some;
         const int l = pass ? __ffsll((unsigned long long)pass) - 1 : 63 - __clzll((long long)some);
         double run = __shfl(upto, max(l - 1, 0), 64);
         if (l == 0) run = 0.0;

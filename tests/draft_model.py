@@ -144,3 +144,63 @@ def keep(cache, seq, rows, path):
                         m = th == s
                         dst[to[m]] = (dst[to[m]] & np.uint8(240 >> s)) | (codes[m] << np.uint8(s))
                     dst[tc], dst[tc + 1] = scales
+
+
+def unit(u):
+    """A random number as the verification takes it: the nearest one in [0, 1), NaN as 0."""
+    below = np.nextafter(np.float32(1), np.float32(0))
+    return np.float32(0) if np.isnan(u) else np.clip(np.float32(u), np.float32(0), below)
+
+
+def lane_scan(v):
+    """Sums of the lanes up to each, in the order of a wave's scan (64 values, 64 bits)."""
+    v = v.copy()
+    for off in (1, 2, 4, 8, 16, 32):
+        v[off:] = v[off:] + v[:-off]
+    return v
+
+
+def choose(w, u):
+    """The first x at which the sum of w(0 .. x) passes u times the sum of all, in the kernel's own order of additions (its
+    weights w in 64 bits, some above 0), and which lanes' sums pass their neighbours' although the lanes have no weight."""
+    vocab = len(w)
+    block = -(-vocab // (256 * 2048)) * 256
+    n = -(-vocab // block)
+    w = np.concatenate([w, np.zeros(n * block - vocab)])
+    lanes = np.zeros((n, 64))
+    for o in range(0, block, 64):
+        lanes += w.reshape(n, block)[:, o:o + 64]
+    for off in (32, 16, 8, 4, 2, 1):
+        lanes = lanes + lanes[:, np.arange(64) ^ off]
+    sums, per = lanes[:, 0], -(-n // 64)
+    own = np.zeros(64)
+    of = [range(min(lane * per, n), min((lane + 1) * per, n)) for lane in range(64)]
+    for lane in range(64):
+        for i in of[lane]:
+            own[lane] += sums[i]
+    upto = lane_scan(own)
+    at = float(unit(u)) * upto[63]
+    some, steps = own > 0, np.diff(upto, prepend=0.0) > 0
+    passes = np.flatnonzero((upto > at) & some)
+    lane = int(passes[0]) if len(passes) else int(np.flatnonzero(some)[-1])
+    run, e = upto[lane - 1] if lane else 0.0, -1
+    for i in of[lane]:
+        if sums[i] == 0:
+            continue
+        if e >= 0:
+            run += sums[e]
+        e = i
+        if run + sums[i] > at:
+            break
+    assert e >= 0
+    token = -1
+    for o in range(e * block, (e + 1) * block, 64):
+        v = w[o:o + 64]
+        to = run + lane_scan(v)
+        here = np.flatnonzero((to > at) & (v > 0))
+        if len(here):
+            return o + int(here[0]), steps & ~some & (upto > at)
+        if (v > 0).any():
+            token = o + int(np.flatnonzero(v)[-1])
+        run = to[63]
+    return token, steps & ~some & (upto > at)
