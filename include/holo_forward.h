@@ -243,11 +243,13 @@ int holo_attention_kv4_draft(const holo_kv4_t *c, int layer, float *out, const f
  * path (device, [rows]) gets the entry's rows that stand, row 0 first, then -1;
  * n_path[s] how many; next[s] the token behind the last of them: the first x at which the
  * sum of w(0 .. x) passes u of row 0 times the sum of all, w = max(p - beta q, 0), or p
- * without the refused tokens (no weight at all: the target's most probable token).  A u outside [0, 1)
- * counts as the nearest number inside, NaN as 0.  Sums are
+ * without the refused tokens (no weight at all: the target's most probable token).  A u
+ * outside [0, 1) counts as the nearest number inside, NaN as 0.  Sums are
  * in 64 bits.  target's rows sum to 1; values that are negative or no finite
  * numbers count as 0.  Tokens outside 0 .. vocab - 1 never stand.  An entry without
- * rows: n_path 0, next -1.  vocab up to 2^24, max_rows up to 1024.  0 or HOLO_EINVAL. */
+ * rows beside others that have some: n_path 0, next -1.  A batch whose `rows` is 0
+ * writes nothing, as every call: n_path and next keep what an earlier step left
+ * there.  vocab up to 2^24, max_rows up to 1024.  0 or HOLO_EINVAL.               */
 #define HOLO_DRAFT_CHOSEN 0
 #define HOLO_DRAFT_DRAWN 1
 #define HOLO_DRAFT_DISTINCT 2
