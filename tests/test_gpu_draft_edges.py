@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+import draft_model as dm
 from kv4_model import Batch
 from test_gpu_draft import MODES, up, verify
 
@@ -26,3 +27,50 @@ def test_verification_without_rows(holo, mode):
     holo.lib().cuda_sync()
     holo.check("no rows")
     assert [o.download(np.int32).tolist() for o in outs] == [[5] * 3, [6] * 3, [7] * 3]
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_verification_at_its_borders_as_written_down(holo, mode):
+    """Outcomes by the formulas, not by the model.  p: 0.25, 0.5, 0.25 at 3, 300, 599; q: all at 300."""
+    print(f"case verify borders by hand {mode}", flush=True)
+    p = np.zeros((4, 600), np.float32)
+    p[:, 3], p[:, 300], p[:, 599] = 0.25, 0.5, 0.25
+    q = np.zeros_like(p)
+    q[:, 300] = 1.0
+    t = [[-1, 0, 0, 1]]
+
+    def call(tokens, u):
+        path, n, after = verify(holo, [4], t, tokens, u, p, q, mode)
+        assert (path[n[0]:] == -1).all()
+        return path[:n[0]].tolist(), int(after[0])
+
+    # row 1 (token 300, u 0.5): 0.5 < 0.5 does not hold, so it is refused; row 2 (token 3, u 0): 0 < 0.25 stands; nothing
+    # follows row 2, and of 0.25, 0.5, 0.25 the second passes 0.5.  Without repeats all of q is gone with 300: 0 < 0.25 * 0
+    # does not hold, and of p - q, 0.25 and 0.25, the second passes 0.25
+    assert call([0, 300, 3, 300], [0.5, 0.5, 0, 0.6]) == (([0], 599) if mode == "distinct" else ([0, 2], 300))
+    # row 1 stands (0.4 < 0.5), then row 3 behind it (0.3 < 0.5); 0.75 of the sum: the third
+    assert call([0, 300, 3, 300], [0.75, 0.4, 0, 0.3]) == ([0, 1, 3], 599)
+    # both refused.  Chosen: 300 again weighs nothing, 3 and 599 are left.  Otherwise p - q leaves the same two
+    assert call([0, 300, 300, 9], [0.25, 0.9, 0.9, 0]) == ([0], 3)
+    assert call([0, 300, 300, 9], [0.5, 0.9, 0.9, 0]) == ([0], 599)
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_every_entry_of_many_is_as_the_model_has_it(holo, mode):
+    """Probabilities of odd numerators, whose sums meet no number drawn: every entry is compared."""
+    print(f"case verify every entry {mode}", flush=True)
+    rng = np.random.default_rng(18)
+    n, t = 2000, [-1, 0, 0, 1]
+    p, q = rng.dirichlet(np.ones(6), 2).astype(np.float32)
+    tokens = rng.integers(0, 6, (n, 4))
+    u = rng.random((n, 4)).astype(np.float32)
+    p4, q4 = np.tile(p, (4, 1)), np.tile(q, (4, 1))
+    path, n_path, after = verify(holo, [4] * n, [t] * n, tokens.ravel(), u.ravel(), np.tile(p, (4 * n, 1)),
+                                 np.tile(q, (4 * n, 1)), mode)
+    path, compared = path.reshape(n, 4), 0
+    for i in range(n):
+        want, token, margin = dm.verify(t, tokens[i], u[i], p4, q4, mode)
+        if margin > 1e-12:
+            compared += 1
+            assert path[i].tolist() == want + [-1] * (4 - len(want)) and after[i] == token and n_path[i] == len(want)
+    assert compared >= 0.95 * n
