@@ -1965,8 +1965,13 @@ int holo_softmax_rows(float *dst, const float *x, int rows, int n, int ldd, int 
     }
     if (rows == 0 || n == 0) return 0;
     const bool by4 = (((uintptr_t)dst | (uintptr_t)x) & 15) == 0 && n % 4 == 0 && ldd % 4 == 0 && ldx % 4 == 0;
+    // (a dimension of a launch has below 2^32 threads: more are cut off, and no error says so)
+    constexpr int kRowsAtOnce = 1 << 21;
     auto run = [&](auto kern, int threads) {
-        hipLaunchKernelGGL(kern, dim3(rows), dim3(threads), 0, stream(), dst, x, n, ldd, ldx, scale);
+        for (int64_t at = 0; at < rows; at += kRowsAtOnce) {
+            const unsigned some = (unsigned)(rows - at < kRowsAtOnce ? rows - at : kRowsAtOnce);
+            hipLaunchKernelGGL(kern, dim3(some), dim3(threads), 0, stream(), dst + at * ldd, x + at * ldx, n, ldd, ldx, scale);
+        }
     };
     // Threads and registers by a row's length: 300 rows of 4096 4.0 us, with 1024 threads 8.4; of
     // 5000 6.6, with 1024 8.8.

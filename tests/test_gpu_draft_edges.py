@@ -74,3 +74,18 @@ def test_every_entry_of_many_is_as_the_model_has_it(holo, mode):
             compared += 1
             assert path[i].tolist() == want + [-1] * (4 - len(want)) and after[i] == token and n_path[i] == len(want)
     assert compared >= 0.95 * n
+
+
+def test_softmax_of_more_rows_than_a_launch_has(holo):
+    """2^24 rows of 256 threads each are 2^32 threads."""
+    print("case softmax 2^24 rows", flush=True)
+    rows, lib = (1 << 24) + 5, holo.lib()
+    x = np.random.default_rng(0).random((rows, 2), dtype=np.float32)
+    dx, dd = up(holo, x), up(holo, np.full(x.shape, -9.0, np.float32))
+    assert lib.holo_softmax_rows(dd.ptr, dx.ptr, rows, 2, 2, 2, 1.0) == 0
+    lib.cuda_sync()
+    holo.check("softmax of many rows")
+    got = dd.download(np.float32).reshape(rows, 2)
+    e = np.exp(x.astype(np.float64))
+    # an exponential, their sum, its reciprocal and a product: 2^-22 at most
+    assert np.abs(got - e / e.sum(1, keepdims=True)).max() <= 2.0 ** -22
