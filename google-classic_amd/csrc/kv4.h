@@ -71,6 +71,15 @@ bool kv4_call_ok(const holo_kv4_t *c, int layer, const holo_batch_t *b);
 bool batch_ok(const holo_batch_t *b);
 bool draft_rows_ok(const holo_batch_t *b, int words);  // an entry's rows have a bit each in so many words
 Kv4View kv4_view(const holo_kv4_t *c, int layer);
+// run(first, n) for the tiles that `take` rows of an entry can lie in, at most 2^23 a launch: a dimension has
+// below 2^32 threads (more are cut off, and no error says so), and take may be a far bound.
+template <typename F>
+inline void kv4_tile_launches(int take, F run)
+{
+    constexpr int kAtOnce = 1 << 23;
+    const int n = (take + 30) / 32 + 1;
+    for (int at = 0; at < n; at += kAtOnce) run(at, n - at < kAtOnce ? n - at : kAtOnce);
+}
 // Rows at p, ld floats from one to the next, of `dim` floats, in 16-byte pieces.
 inline bool rows_ok(const void *p, int ld, int64_t dim) { return p && !((uintptr_t)p & 15) && ld % 4 == 0 && ld >= dim; }
 

@@ -47,14 +47,15 @@ struct VWords {
 // 5.1.)
 template <int NB>
 __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, const float *k, const float *v, int ldk,
-                                                    int ldv)
+                                                    int ldv, int first)
 {
     constexpr int HD = 32 * NB;
     __shared__ __align__(16) uint8_t lv[32 * HD];
     const Kv4Entry e = kv4_entry(c, b, blockIdx.z);
     const int kvh = blockIdx.y, from = e.len - e.rows;  // position of the entry's first row
-    if ((int)blockIdx.x > (e.take + 30) / 32) return;  // (so that 32 t stays an int)
-    const int t = (max(from, 0) >> 5) + blockIdx.x, p0 = 32 * t;
+    const int nth = first + (int)blockIdx.x;  // of the entry's tiles
+    if (nth > (e.take + 30) / 32) return;     // (so that 32 t stays an int)
+    const int t = (max(from, 0) >> 5) + nth, p0 = 32 * t;
     // the tile's positions in the batch: lo .. hi - 1
     const int lo = max(from - p0, 0), hi = min(min(from + e.take, e.len) - p0, 32);
     if (lo >= hi) return;
@@ -80,7 +81,8 @@ __global__ __launch_bounds__(256) void kv4_append_k(Kv4View c, holo_batch_t b, c
 // large copy's rate), 32 single rows 3.0.
 
 template <int NB>
-__global__ __launch_bounds__(256) void kv4_read_k(Kv4View c, holo_batch_t b, float *k, float *v, int ldk, int ldv)
+__global__ __launch_bounds__(256) void kv4_read_k(Kv4View c, holo_batch_t b, float *k, float *v, int ldk, int ldv,
+                                                  int first)
 {
     constexpr int HD = 32 * NB;
     __shared__ __align__(16) uint8_t lv[32][HD];
@@ -88,8 +90,9 @@ __global__ __launch_bounds__(256) void kv4_read_k(Kv4View c, holo_batch_t b, flo
     const int kvh = blockIdx.y, from = e.len - e.rows;
     // rows before position 0 and of a tile without a page are zeros: the tiles are
     // counted from the one of `from`, which may be negative
-    if ((int)blockIdx.x > (e.take + 30) / 32) return;
-    const int t = (from >> 5) + (int)blockIdx.x, p0 = 32 * t;
+    const int nth = first + (int)blockIdx.x;
+    if (nth > (e.take + 30) / 32) return;
+    const int t = (from >> 5) + nth, p0 = 32 * t;
     const int lo = max(from - p0, 0), hi = min(from + e.take - p0, 32);
     if (lo >= hi) return;
     const uint8_t *tile = t < 0 ? nullptr : kv4_tile<NB>(c, e, kvh, t);
@@ -440,8 +443,11 @@ int holo_kv4_append(const holo_kv4_t *c, int layer, const float *k, const float 
         return rejected("holo_kv4_append: null or misaligned rows, or rows that overlap");
     const Kv4View w = kv4_view(c, layer);
     const int take = b->max_rows < b->rows ? b->max_rows : b->rows;
-    const dim3 grid((unsigned)(take + 30) / 32 + 1, c->n_kv_heads, b->n_seqs);
-    auto run = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream(), w, *b, k, v, ldk, ldv); };
+    auto run = [&](auto kern) {
+        kv4_tile_launches(take, [&](int first, int n) {
+            hipLaunchKernelGGL(kern, dim3(n, c->n_kv_heads, b->n_seqs), dim3(256), 0, stream(), w, *b, k, v, ldk, ldv, first);
+        });
+    };
     switch (c->head_dim) {
     case 32: run(kv4_append_k<1>); break;
     case 64: run(kv4_append_k<2>); break;
@@ -461,8 +467,11 @@ int holo_kv4_read(const holo_kv4_t *c, int layer, float *k, float *v, int ldk, i
         return rejected("holo_kv4_read: null or misaligned rows, or rows that overlap");
     const Kv4View w = kv4_view(c, layer);
     const int take = b->max_rows < b->rows ? b->max_rows : b->rows;
-    const dim3 grid((unsigned)(take + 30) / 32 + 1, c->n_kv_heads, b->n_seqs);
-    auto run = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream(), w, *b, k, v, ldk, ldv); };
+    auto run = [&](auto kern) {
+        kv4_tile_launches(take, [&](int first, int n) {
+            hipLaunchKernelGGL(kern, dim3(n, c->n_kv_heads, b->n_seqs), dim3(256), 0, stream(), w, *b, k, v, ldk, ldv, first);
+        });
+    };
     switch (c->head_dim) {
     case 32: run(kv4_read_k<1>); break;
     case 64: run(kv4_read_k<2>); break;

@@ -52,7 +52,7 @@ __device__ __forceinline__ void turn_pair(float &x, float &y, double cs, double 
 // the read back, through them 39.7).  Four sequences of 8 rows 6.6: lengths, page, rows, angles one
 // after the other.  (One pair a thread 40 us; the pairs' layout not a template, 55 with the read back.)
 template <int NB, bool WIDE, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void kv4_append_rope_k(Kv4View c, holo_batch_t b, RopeRows a)
+__global__ __launch_bounds__(256) void kv4_append_rope_k(Kv4View c, holo_batch_t b, RopeRows a, int first)
 {
     constexpr int HD = 32 * NB, N = WIDE ? 4 : 1, P = HD / (2 * N), GROUPS = 256 / P, KS = HD + 4;
     typedef float vec __attribute__((ext_vector_type(N)));
@@ -62,8 +62,9 @@ __global__ __launch_bounds__(256) void kv4_append_rope_k(Kv4View c, holo_batch_t
     const int kvh = blockIdx.y % c.n_kv_heads, part = blockIdx.y / c.n_kv_heads;
     const int G = a.n_heads / c.n_kv_heads, h0 = part * kRopeHeads, heads = min(G - h0, kRopeHeads);
     const int from = e.len - e.rows;  // position of the entry's first row, which may be negative
-    if ((int)blockIdx.x > (e.take + 30) / 32) return;
-    const int t = (from >> 5) + (int)blockIdx.x, p0 = 32 * t;
+    const int nth = first + (int)blockIdx.x;  // of the entry's tiles
+    if (nth > (e.take + 30) / 32) return;
+    const int t = (from >> 5) + nth, p0 = 32 * t;
     const int lo = max(from - p0, 0), hi = min(from + e.take - p0, 32), n = hi - lo;
     if (n <= 0) return;
     const int64_t row0 = (int64_t)e.first + p0 - from;
@@ -199,10 +200,13 @@ int holo_kv4_append_rope(const holo_kv4_t *c, int layer, const holo_rope_t *r, c
     }
     const Kv4View w = kv4_view(c, layer);
     const int take = b->max_rows < b->rows ? b->max_rows : b->rows;
-    const dim3 grid((unsigned)(take + 30) / 32 + 1, (unsigned)(parts * c->n_kv_heads), b->n_seqs);
     const RopeRows a{*r, q, k, v, q_out, k_out, ldq, ldk, ldv, ldqo, ldko, n_heads, depth};
     const bool wide = r->dims % 8 == 0;
-    auto run = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream(), w, *b, a); };
+    auto run = [&](auto kern) {
+        kv4_tile_launches(take, [&](int first, int n) {
+            hipLaunchKernelGGL(kern, dim3(n, (unsigned)(parts * c->n_kv_heads), b->n_seqs), dim3(256), 0, stream(), w, *b, a, first);
+        });
+    };
     auto pick = [&](auto nb) {
         if (r->interleaved) wide ? run(kv4_append_rope_k<nb, true, true>) : run(kv4_append_rope_k<nb, false, true>);
         else wide ? run(kv4_append_rope_k<nb, true, false>) : run(kv4_append_rope_k<nb, false, false>);

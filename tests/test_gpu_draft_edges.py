@@ -1,9 +1,11 @@
 """Drafted tokens on the GPU: calls at the edges of what they take."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import draft_model as dm
-from kv4_model import Batch
+from kv4_model import Batch, Cache, OnDevice, quantise, values
 from test_gpu_draft import MODES, up, verify
 
 pytestmark = pytest.mark.gpu
@@ -89,3 +91,32 @@ def test_softmax_of_more_rows_than_a_launch_has(holo):
     e = np.exp(x.astype(np.float64))
     # an exponential, their sum, its reciprocal and a product: 2^-22 at most
     assert np.abs(got - e / e.sum(1, keepdims=True)).max() <= 2.0 ** -22
+
+
+@pytest.mark.parametrize("bound", [(1 << 29) - 63, (1 << 29) - 62, (1 << 29) - 30, 1 << 30, 0x7FFFF000])
+def test_rows_under_far_bounds(holo, bound):
+    """max_rows and rows are bounds: 70 rows go in and come back whatever they are, 2^32 threads and more among them."""
+    print(f"case far bound {bound}", flush=True)
+    hd, n, lib = 32, 70, holo.lib()
+    rng = np.random.default_rng(2)
+    k, v = rng.standard_normal((2, n, hd)).astype(np.float32)
+    for rotated in (False, True):
+        c = Cache(hd, 32, 1, 1, 3, 1, 3, fill=0)
+        c.table[0], c.len[0] = (2, 0, 1), n
+        dev = OnDevice(holo, c)
+        dk, dv = up(holo, k), up(holo, v)
+        b = Batch(holo, [n])
+        b.desc.max_rows = b.desc.rows = bound
+        if rotated:
+            freq = up(holo, np.zeros(hd // 2))  # no angle: rows as they are
+            rope = holo.Rope(freq=freq.ptr, dims=hd, interleaved=0, scale=1.0)
+            assert lib.holo_kv4_append_rope(dev.ref, 0, C.byref(rope), None, dk.ptr, dv.ptr, 0, hd, hd, None, None, 0, 0, 0,
+                                            None, b.ref) == 0
+        else:
+            assert lib.holo_kv4_append(dev.ref, 0, dk.ptr, dv.ptr, hd, hd, b.ref) == 0
+        out = [up(holo, np.full((n, hd), -9.0, np.float32)) for _ in range(2)]
+        assert lib.holo_kv4_read(dev.ref, 0, out[0].ptr, out[1].ptr, hd, hd, b.ref) == 0
+        lib.cuda_sync()
+        holo.check("far bounds")
+        for got, x in zip(out, (k, v)):
+            assert np.array_equal(got.download(np.float32).reshape(n, hd), values(*quantise(x)))
