@@ -111,14 +111,17 @@ __global__ __launch_bounds__(1024) void softmax_k(float *dst, const float *x, in
     for (int i = threadIdx.x; i < n; i += blockDim.x) dst[i] *= inv;
 }
 
-// e^t for t <= 0 (0 below -150, NaN for NaN): t log2(e) in two parts, the first by the
-// hardware's 2^h, the second, below 2^-16, by 1 + l ln(2).  Within 2^-22 of itself.
+// e^t for t <= 0 (NaN for NaN): t log2(e) less its nearest integer n, |f| <= 1/2, by the
+// hardware's 2^f, then times 2^n, which rounds once more only below a float's normal range.
+// Off by 2^-23.4 at most, 2.2e-8 on average; t log2(e) in two parts, the second by 1 + l ln(2),
+// which flushes what lies below the normal range: 2^-22.8, 2.9e-8 (416 rows of 32000 the same time,
+// five of 128256 25.0 us for 26.2).  expf is as near, and five rows of 32000 take 8.4 us for 7.6.
 __device__ __forceinline__ float exp_down(float t)
 {
     t = t < -150.f ? -150.f : t;
-    const float h = t * 1.44269504f, l = fmaf(t, 1.92596299e-8f, fmaf(t, 1.44269504f, -h));
-    const float e = __builtin_amdgcn_exp2f(h);
-    return fmaf(e, l * 0.693147181f, e);
+    const float n = rintf(t * 1.44269504f);
+    const float f = fmaf(t, 1.92596299e-8f, fmaf(t, 1.44269504f, -n));
+    return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
 }
 
 // Each of many rows: softmax(scale (x - max x)), a row of nothing but -infinity zeros.

@@ -93,6 +93,28 @@ def test_softmax_of_more_rows_than_a_launch_has(holo):
     assert np.abs(got - e / e.sum(1, keepdims=True)).max() <= 2.0 ** -22
 
 
+def test_small_exponentials_of_a_row(holo):
+    """Rows of 0 and t below -17: their sum rounds to 1, so the second value is e^t itself, down to a float's least step."""
+    print("case softmax exponentials", flush=True)
+    rng, n, lib = np.random.default_rng(4), 1 << 18, holo.lib()
+    x = np.zeros((2 * n, 2), np.float32)
+    x[:n, 1], x[n:, 1] = rng.uniform(-87.3, -17, n), rng.uniform(-110, -87.3, n)
+    x[-1, 1], x[-2, 1] = -np.inf, -3e38
+    dx, dd = up(holo, x), up(holo, np.full(x.shape, -9.0, np.float32))
+    assert lib.holo_softmax_rows(dd.ptr, dx.ptr, len(x), 2, 2, 2, 1.0) == 0
+    lib.cuda_sync()
+    holo.check("small exponentials")
+    got = dd.download(np.float32).reshape(-1, 2).astype(np.float64)
+    want = np.exp(x[:, 1].astype(np.float64))
+    assert (got[:, 0] == 1).all()
+    # the hardware's 2^f is within a unit of the last place, 2^-23 of itself; f within 2^-25, which counts times ln 2; below
+    # the normal range half a step of 2^-149 for the last rounding
+    off = np.abs(got[:, 1] - want)
+    assert (off[:n] <= (2.0 ** -23 + 2.0 ** -25) * want[:n]).all()
+    assert (off[n:] <= (2.0 ** -23 + 2.0 ** -25) * want[n:] + 2.0 ** -150).all()
+    assert (got[-2:, 1] == 0).all()
+
+
 @pytest.mark.parametrize("bound", [(1 << 29) - 63, (1 << 29) - 62, (1 << 29) - 30, 1 << 30, 0x7FFFF000])
 def test_rows_under_far_bounds(holo, bound):
     """max_rows and rows are bounds: 70 rows go in and come back whatever they are, 2^32 threads and more among them."""
