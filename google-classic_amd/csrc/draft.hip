@@ -1,10 +1,7 @@
 // draft.hip -- drafted tokens (holo_forward.h): what the rows of a tree follow, and
 // which of them stand against the target's probabilities.
-#include "block_reduce.h"
 #include "kv4.h"
 #include "stream_scratch.h"
-
-#include <float.h>
 
 namespace holo {
 
