@@ -108,3 +108,26 @@ def test_not_touched_by_what_a_row_does_not_see(holo, hd, heads, rows):
     for form, got in forms(holo, OnDevice(holo, c), q, [rows], heads, mask, [0]).items():
         got = got.reshape(rows, heads, hd)
         assert np.array_equal(np.isnan(got), ~ok) and normwise(got[ok], want[ok]) <= TOL, form
+
+
+@pytest.mark.parametrize("hd,heads,n_kv", [(128, 2, 1), (32, 4, 2)])
+def test_more_pages_than_lanes(holo, hd, heads, n_kv):
+    """A wave holds 64 entries of the table at a time: ranges of up to 141 pages of 32 positions, some of them missing."""
+    print(f"case columns pages {hd} {heads}/{n_kv}", flush=True)
+    rng = np.random.default_rng(hd)
+    lens, rows, seqs = [4500, 2080, 2047], [9, 20, 33], [0, 1, 2]
+    c = Cache(hd, 32, 1, n_kv, 280, 3, 141)
+    pages(c, lens, rng)
+    c.table[0, [3, 64, 100]] = -1, 280, -7
+    c.pool[:] = rng.integers(0, 256, c.pool.shape, dtype=np.uint8)
+    f = c.pool[..., 32 * hd:].view(np.uint16)  # scales of 0.5 to 2, either sign, in the cache's 8 significant bits
+    f[:] = (f & 0x83F8) | (0x3800 + (f & 0x0400))
+    dev = OnDevice(holo, c)
+    seen = [dm.seen_rows(dm.tree(rng, n, 2)) for n in rows]
+    q = (0.1 * rng.standard_normal((sum(rows), heads * hd))).astype(np.float32)
+    want = dm.want_attention(c, 0, q, rows, seqs, heads, seen)
+    mask = np.concatenate([dm.words(s, 2) for s in seen])
+    got = forms(holo, dev, q, rows, heads, mask, seqs)
+    got["16 columns"] = attention(holo, dev, 0, q, rows, heads, mask, seqs=seqs)
+    for form, x in got.items():
+        assert normwise(x, want) <= TOL, form
