@@ -14,8 +14,9 @@
 // TFLOP/s of scores and values, twice that on the matrix cores for the halves: 0.93 of the
 // 1.14 PFLOP/s that a large f16 product reaches here.  Matrix and vector instructions of a
 // SIMD's two waves hardly overlap: they issue in 40% and 53% of the cycles.  64 x 5 rows of up to
-// 8192 140-146 us, 3.2 TB/s, 20 of 32 columns in use, 33% and 44%; 16 x 26 of up to 4096 53, the
-// longest sequences' workgroups (mean 67 tiles, the longest 128); 5 rows of 517 positions 9.0,
+// 8192 140-146 us, 3.2 TB/s, 20 of 32 columns in use, 33% and 44%; 16 x 26 of up to 4096 53-57, the
+// longest sequences' workgroups (mean 67 tiles, the longest 128).  Both with the longest entries
+// first: workgroups start in the caller's order, and in others it is 149-154 and 63-75.  5 rows of 517 positions 9.0,
 // a chain of five tiles of 1.05 each and the launch.
 //
 // Tried: the tiles unpacked once into LDS for 64 or 128 columns of four waves, a tile
@@ -499,7 +500,11 @@ static int run_draft(Draft d)
     // For two workgroups a CU, or where the sequences' ends leave more ranges than that, one
     // and a half (16 sequences of 8 rows at up to 4096: 31.1 us, for two 36.6).  Worth
     // the join where a sequence gets some 36 tiles shorter (max_len is all that is known of them): 8 rows
-    // at 2000 (45) 19.4 -> 18.9 in eight sequences, 5 rows (21) 20.2 -> 24.6 in sixteen.
+    // at 2000 (45) 19.4 -> 18.9 in eight sequences, 5 rows (21) 20.2 -> 24.6 in sixteen.  Between them,
+    // by tiles and us whole and cut: 31 (8 x 8 at 1500) 16.9, 18.7; 32 (4 x 5 at 1200) 14.5, 16.6; 37
+    // (1 x 5) 14.4, 13.4; 42 (1 x 26 at 1500) 16.4, 17.1; 43 (16 x 8 at 2048 to 4096, shuffled) 36.8,
+    // 38.7; 63 (8 x 8 at 3000) 27.5, 22.7.  A far max_len cuts whatever there is: 5 rows of 517
+    // positions 12.3 for 9.5.
     d.cut = n == 1 ? 2 * num_cus() : 3 * num_cus() / 2;
     const bool cuts = n <= 1024 && tiles * (d.cut - n * groups) > (int64_t)36 * d.cut;
     // (ranges: tiles / chunk of them and one more an entry at most)
@@ -545,7 +550,9 @@ static int run_draft(const Draft &d)
 {
     // 16 columns a workgroup; 32, which unpack a tile once for both halves but take twice as long
     // for it, where that makes 256 tiles or more for each of two workgroups a CU (64 x 5 at up to 8192, 512 tiles: 146
-    // us, with 16 columns 178; 16 x 26 at up to 4096, 224 tiles: 55.4 and 52.9).
+    // us, with 16 columns 178; 16 x 26 at up to 4096, 224 tiles: 55.4 and 52.9).  With the entries
+    // shuffled, us of 16 and 32 columns: 256 tiles 104 and 84 (64 x 5 at 4096), 276 104 and 91, 329 127
+    // and 96; but 32 are ahead below the bound too, 188 83 and 67 (64 x 8 at 3000), 224 77 and 57.
     const int64_t cols = (int64_t)d.a.b.max_rows * (d.a.n_heads / d.a.c.n_kv_heads);
     const int64_t work = (int64_t)d.a.b.n_seqs * d.a.c.n_kv_heads * ((cols + 15) / 16) * ((d.a.b.max_len + 31) / 32);
     return cols > 16 && work >= (int64_t)256 * 2 * num_cus() ? run_draft<NB, 2>(d) : run_draft<NB, 1>(d);

@@ -59,10 +59,10 @@ __global__ __launch_bounds__(1024) void draft_plan_k(const int *parent, int *dep
 // all that a refusal costs.
 //
 // What bounds it: latency.  64 chains of 5 rows, 32000 tokens, 16.4 MB of the rows that the
-// walks end at (3.4 us at a large copy's rate): 12.8-13.1 us, two launches of 5 and 4.4 with loads
+// walks end at (3.4 us at a large copy's rate): 12.7-13.1 us (chosen 13.6; 128256 tokens 20.7), two launches of 5 and 4.4 with loads
 // that depend on each other (rows, tokens, probabilities; then the row); with one workgroup an entry for
-// all of it 42.  16 trees of up to 26 rows 28-32 (78): the second launch goes from refusal to
-// refusal, some 4 us each, half of it 64-bit arithmetic; with the row's probabilities kept in registers
+// all of it 42.  16 trees of up to 26 rows 26-32 (78; chosen, where a refusal costs no sum, 13.8;
+// of 128256 tokens 83-97): the second launch goes from refusal to refusal, some 4 us each, half of it 64-bit arithmetic; with the row's probabilities kept in registers
 // the compiler spills them (50-57).
 
 struct Verify {

@@ -50,7 +50,9 @@ __device__ __forceinline__ void turn_pair(float &x, float &y, double cs, double 
 // trace; vector instructions (a third in 64 bits) issue in about a third of the cycles, the rest is
 // memory, the rows written among it at the launch's end (past the caches they take 37.4 us with
 // the read back, through them 39.7).  Four sequences of 8 rows 6.6: lengths, page, rows, angles one
-// after the other.  (One pair a thread 40 us; the pairs' layout not a template, 55 with the read back.)
+// after the other.  (Of other
+// dims, one pair a thread: from call to call 98 dims take 25.7 us in halves and 32.0 interleaved,
+// 96 dims 25.0 and 28.2.  The pairs' layout not a template, 55 with the read back.)
 template <int NB, bool WIDE, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void kv4_append_rope_k(Kv4View c, holo_batch_t b, RopeRows a, int first)
 {

@@ -127,8 +127,11 @@ __device__ __forceinline__ float exp_down(float t)
 // Each of many rows: softmax(scale (x - max x)), a row of nothing but -infinity zeros.
 // A workgroup takes a row; up to 4 R values a thread stay in registers, what is past
 // them is read twice: a running maximum and sum, then the values.  V: values of a load
-// (4 where the rows are 16-byte aligned).  416 rows of 32000, 106 MB, 22.6 us, 4.7 TB/s
-// (a large copy 4.8-5.2); five such rows 6.8: a row's loads and exponentials on one CU.
+// (4 where the rows are 16-byte aligned; 416 rows of 50257 66.6 us, of 50256 49.5).  416 rows of
+// 32000, 106 MB, 22.8-24.2 us, 4.4-4.7 TB/s (a large copy 4.8-5.2); five such rows 7.5-7.8: a row's
+// loads and exponentials on one CU.  Past 65536 values half a row is read twice, and fewer rows
+// than CUs leave the others idle: 100 of 128256 39 us, 103 MB; 416 of them 110-118, 427 MB.
+// A row is off by 6e-8 to 1.1e-7 normwise (100 to 128256 values), most of it the sum's.
 template <int T, int R, int V>
 __global__ __launch_bounds__(T) void softmax_rows_k(float *dst, const float *x, int n, int ldd, int ldx, float scale)
 {
